@@ -18,7 +18,7 @@ VT_STATIC_SCRATCH_BYTES = 24 << 20
 VT_STEP_OVERLAP = 1
 VT_STEP_EARLY_KV = 2
 VT_STEP_CLEAN_SCRATCH = 4
-VT_KV_BF16, VT_KV_FP8_E4M3 = 0, 1
+VT_KV_BF16, VT_KV_FP8_E4M3, VT_KV_INT4 = 0, 1, 2
 
 
 class VTensorError(RuntimeError):
@@ -79,6 +79,8 @@ def _load():
                               vp, vp, vp]),
         "vt_kv_scales": (c_int, [vp, c_int64, c_int, c_int, c_int, vp, vp]),
         "vt_kv_widen": (c_int, [vp, vp, vp, vp, c_int, c_int, c_int, c_int, vp, vp, vp, vp, vp]),
+        "vt_kv_row_bytes": (c_int, [c_int, c_int, c_int, POINTER(sz)]),
+        "vt_kv_dequant": (c_int, [vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_int, vp, vp, vp, vp, vp]),
         "vt_rope_append": (c_int, [vp, vp, c_int64, c_int, vp, vp, c_int64, c_int64, vp, c_int, c_int, vp, vp, vp, vp,
                                    vp, vp, c_int, c_int, c_int, c_int, c_int, vp, vp, ctypes.c_uint, vp]),
         "vt_ar_buffer_bytes": (c_int, [sz, POINTER(sz)]),

@@ -52,9 +52,11 @@ class VTensorCacheEngine:
                  cache_dtype="auto", cache_seqs=0, cache_tokens=0, device="cuda"):
         self.num_layers, self.num_kv_heads, self.head_size = num_layers, num_kv_heads, head_size
         self.cache_dtype = cache_dtype
-        self.dtype_size = 1 if cache_dtype in ("fp8", "fp8_e4m3") else 2
+        # bytes of an element; 0 for the 4-bit cache, whose rows also hold their group scales
+        self.dtype_size = {"fp8": 1, "fp8_e4m3": 1, "int4": 0}.get(cache_dtype, 2)
         self.device = torch.device(device)
-        self.token_size = num_kv_heads * head_size * self.dtype_size
+        self.token_size = (ops.kv_row_bytes(num_kv_heads, head_size, cache_dtype) if cache_dtype == "int4"
+                           else num_kv_heads * head_size * self.dtype_size)
         # cache_engine.py:55-57: room for max_num_batched_tokens rows, whole chunks
         self.max_context_size = _round_up(max_num_batched_tokens * self.token_size, vmmAllocator.granularitySize)
         self.kv_batch_stride = self.max_context_size
@@ -155,7 +157,7 @@ def prepare_step_host(meta: VTensorMetadata, engine: VTensorCacheEngine):
     meta.kvcache_segment = segs
     meta.k_cache_segment_ptr_list = engine.k_cache_ptr
     meta.v_cache_segment_ptr_list = engine.v_cache_ptr
-    kv_size = meta.kv_num_heads * meta.kv_head_size * meta.kv_elem_size
+    kv_size = engine.token_size if engine.cache_dtype == "int4" else meta.kv_num_heads * meta.kv_head_size * meta.kv_elem_size
     decode = meta.num_prefills == 0
     if decode:
         if vmmAllocator.query_cycle(slots):

@@ -320,8 +320,7 @@ attn_flat_kernel(AttnParams p) {
               dst[W<NB>::dim_of(mb, 0, r4)] = __float2bfloat16(st.o[nb][mb][e] * inv);
               dst[W<NB>::dim_of(mb, 1, r4)] = __float2bfloat16(st.o[nb][mb][2 + e] * inv);
             }
-            if (p.lse && r4 == 0)
-              p.lse[pc.b * p.h + hq] = (st.mrun[nb][e] + log2f(st.lrun[nb][e])) * 0.6931471805599453f;
+            if (r4 == 0) write_stats(p, pc.b * p.h + hq, st.mrun[nb][e], st.lrun[nb][e]);
           }
         }
       }
@@ -446,11 +445,12 @@ bool attn_flat_supports(int batch, int h, int kvh, int kv_dtype) {
   return false;
 }
 
-int flat_consumer_warps(int kv_dtype) { return kv_dtype == VT_KV_FP8_E4M3 ? 8 : 4; }
+int flat_consumer_warps(int kv_dtype) { return kv_dtype == VT_KV_BF16 ? 4 : 8; }
 
 // Largest grid launch() uses for this problem: the scratch holds two piece slots per CTA.
 int flat_max_ctas(int h, int kvh, int kv_dtype) {
   const bool nb1 = (h / kvh) <= 8;
+  if (kv_dtype == VT_KV_INT4) return (nb1 ? 2 : 1) * kFlatSms;
   const int per_sm = kv_dtype == VT_KV_FP8_E4M3 ? (nb1 ? FlatCfg<WarpAttnF8, 1>::kCtasPerSm : FlatCfg<WarpAttnF8, 2>::kCtasPerSm)
                                                 : (nb1 ? FlatCfg<WarpAttn, 1>::kCtasPerSm : FlatCfg<WarpAttn, 2>::kCtasPerSm);
   return per_sm * kFlatSms;

@@ -57,6 +57,12 @@ __device__ __forceinline__ int owner_of(long long tau, long long total, int n_ct
   return static_cast<int>(((tau + 1) * n_ctas - 1) / total);
 }
 
+// Softmax statistics of one (entry, q head): log-sum-exp for the caller, (max, sum) for the weight accumulation.
+__device__ __forceinline__ void write_stats(const AttnParams &p, int row, float m, float l) {
+  if (p.lse) p.lse[row] = (m + log2f(l)) * 0.6931471805599453f;
+  if (p.ml) *reinterpret_cast<float2 *>(p.ml + 2 * row) = make_float2(m, l);
+}
+
 // Merge of one stream by the CTA that drew its last ticket.  The caller has published its
 // own piece and passed a CTA-wide barrier; every consumer warp of the CTA calls this.
 // kCWarps / HS / R / HEADS describe the scratch layout ([cta][2 slots][kCWarps][HEADS] rows;
@@ -145,7 +151,7 @@ __device__ __forceinline__ void merge_stream(const AttnParams &p, const Piece &p
     packed.x = pack_bf16(acc.x * inv, acc.y * inv);
     packed.y = pack_bf16(acc.z * inv, acc.w * inv);
     *reinterpret_cast<uint2 *>(out + pc.b * p.out_stride + hq * kHeadDim + lane * 4) = packed;
-    if (p.lse && lane == 0) p.lse[pc.b * p.h + hq] = (M + log2f(L)) * 0.6931471805599453f;
+    if (lane == 0) write_stats(p, pc.b * p.h + hq, M, L);
   }
 }
 

@@ -8,6 +8,7 @@
 
 #include "../../include/vtensor.h"
 #include "vt_device.cuh"
+#include "vt_int4.cuh"
 #include "vt_kernels.h"
 
 namespace vt {
@@ -70,7 +71,7 @@ static size_t flat_counter_bytes(int batch, int kvh) {
 }
 static size_t flat_workspace_bytes(int batch, int h, int kvh, int kv_dtype, bool worst_case = false) {
   const int heads = (!worst_case && (h / kvh) <= 8) ? 8 : 16;
-  const int warps = worst_case ? 8 : flat_consumer_warps(kv_dtype);
+  const int warps = worst_case ? 8 : flat_consumer_warps(kv_dtype);   // 4-bit: 8, as fp8
   const int ctas = worst_case ? kFlatMaxCtas : flat_max_ctas(h, kvh, kv_dtype);
   return kStatusBytes + flat_counter_bytes(batch, kvh) +
          static_cast<size_t>(ctas) * 2 * warps * heads * kFlatPartRow * sizeof(float);
@@ -103,6 +104,13 @@ int plan_attn(int batch, int h, int kvh, int max_seq_len, int kv_dtype, int num_
   // Tensor-core engine wherever it applies (bf16 KV) — on the flat persistent
   // schedule unless the caller asks for explicit splits — SIMT otherwise (fp8 KV).
   (void)g;
+  if (kv_dtype == VT_KV_INT4) {   // one engine, on the persistent schedule; batches beyond its table run in parts
+    plan->variant = 2;
+    plan->part_tokens = max_seq_len;
+    plan->max_parts = 1;
+    plan->ws_bytes = flat_workspace_bytes(batch, h, kvh, kv_dtype);
+    return VT_OK;
+  }
   plan->variant = attn_mma_supports(h, kvh, kv_dtype) ? 1 : 0;
   if (num_splits == 0 && attn_flat_supports(batch, h, kvh, kv_dtype)) plan->variant = 2;
   // Tuning override (vt_attn_set_tuning, or the VT_ATTN_VARIANT / VT_ATTN_PART_TOKENS
@@ -158,12 +166,13 @@ int vt_append(const void *key, const void *value, int64_t key_stride, int64_t va
   if (batch == 0) return VT_OK;
   if (!key || !value || !k_table || !v_table || !byte_off || !slot_ids) return VT_ERR_INVALID;
   if (d != vt::kHeadDim) return VT_ERR_UNSUPPORTED;
-  if (kv_dtype != VT_KV_BF16 && kv_dtype != VT_KV_FP8_E4M3) return VT_ERR_UNSUPPORTED;
-  if (kv_dtype == VT_KV_FP8_E4M3 && (!k_scale || !v_scale)) return VT_ERR_INVALID;
+  if (kv_dtype != VT_KV_BF16 && kv_dtype != VT_KV_FP8_E4M3 && kv_dtype != VT_KV_INT4) return VT_ERR_UNSUPPORTED;
+  if (kv_dtype != VT_KV_BF16 && (!k_scale || !v_scale)) return VT_ERR_INVALID;
   if (max_seq_len > 1 && (!seq_lens || !cache_seq_lens)) return VT_ERR_INVALID;
   if (key_stride < static_cast<int64_t>(kvh) * d || value_stride < static_cast<int64_t>(kvh) * d) return VT_ERR_INVALID;
   vt::AppendParams p{key, value, key_stride, value_stride, k_table, v_table, byte_off, slot_ids,
                      seq_lens, cache_seq_lens, max_seq_len, batch, kvh, k_scale, v_scale};
+  if (kv_dtype == VT_KV_INT4) return vt::launch_append_int4(p, static_cast<cudaStream_t>(stream));
   return vt::launch_append(p, kv_dtype, static_cast<cudaStream_t>(stream));
 }
 
@@ -182,6 +191,30 @@ int vt_kv_widen(const uint64_t *k_table, const uint64_t *v_table, const int64_t 
   if (d != vt::kHeadDim) return VT_ERR_UNSUPPORTED;
   vt::KvWidenParams p{k_table, v_table, slot_ids, seq_lens, k_out, v_out, batch, kvh, k_scale, v_scale};
   return vt::launch_kv_widen(p, max_seq_len, static_cast<cudaStream_t>(stream));
+}
+
+int vt_kv_row_bytes(int kvh, int d, int kv_dtype, size_t *bytes) {
+  if (!bytes || kvh <= 0) return VT_ERR_INVALID;
+  if (d != vt::kHeadDim) return VT_ERR_UNSUPPORTED;
+  switch (kv_dtype) {
+    case VT_KV_BF16: *bytes = static_cast<size_t>(kvh) * d * 2; return VT_OK;
+    case VT_KV_FP8_E4M3: *bytes = static_cast<size_t>(kvh) * d; return VT_OK;
+    case VT_KV_INT4: *bytes = vt::int4_row_bytes(kvh); return VT_OK;
+    default: return VT_ERR_UNSUPPORTED;
+  }
+}
+
+int vt_kv_dequant(const uint64_t *k_table, const uint64_t *v_table, const int64_t *slot_ids, const int32_t *seq_lens,
+                  const int32_t *row_start, int batch, int kvh, int d, int max_seq_len, int kv_dtype,
+                  const float *k_scale, const float *v_scale, void *k_out, void *v_out, void *stream) {
+  if (batch < 0 || kvh <= 0 || max_seq_len < 0) return VT_ERR_INVALID;
+  if (d != vt::kHeadDim || (kv_dtype != VT_KV_FP8_E4M3 && kv_dtype != VT_KV_INT4)) return VT_ERR_UNSUPPORTED;
+  if (batch == 0 || max_seq_len == 0) return VT_OK;
+  if (!slot_ids || !seq_lens || !row_start || (!k_out && !v_out)) return VT_ERR_INVALID;
+  if ((k_out && (!k_table || !k_scale)) || (v_out && (!v_table || !v_scale))) return VT_ERR_INVALID;
+  if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return VT_ERR_INVALID;
+  vt::KvDequantParams p{k_table, v_table, slot_ids, seq_lens, row_start, batch, kvh, k_scale, v_scale, k_out, v_out};
+  return vt::launch_kv_dequant(p, max_seq_len, kv_dtype, static_cast<cudaStream_t>(stream));
 }
 
 int vt_decode_attn_workspace_bytes(int batch, int h, int d, int max_seq_len, size_t *bytes) {
@@ -204,8 +237,13 @@ static int decode_attn_impl(void *out, int64_t out_stride, const void *q, int64_
   if (d != vt::kHeadDim || h % kvh != 0) return VT_ERR_UNSUPPORTED;
   const int g = h / kvh;
   if (g != 1 && g != 2 && g != 4 && g != 8 && g != 16) return VT_ERR_UNSUPPORTED;
-  if (kv_dtype != VT_KV_BF16 && kv_dtype != VT_KV_FP8_E4M3) return VT_ERR_UNSUPPORTED;
-  if (kv_dtype == VT_KV_FP8_E4M3 && (!k_scale || !v_scale)) return VT_ERR_INVALID;
+  if (kv_dtype != VT_KV_BF16 && kv_dtype != VT_KV_FP8_E4M3 && kv_dtype != VT_KV_INT4) return VT_ERR_UNSUPPORTED;
+  if (kv_dtype != VT_KV_BF16 && (!k_scale || !v_scale)) return VT_ERR_INVALID;
+  if (kv_dtype == VT_KV_INT4) {
+    if (num_splits > 1) return VT_ERR_UNSUPPORTED;   // one schedule only
+    num_splits = 0;
+    if ((reinterpret_cast<uintptr_t>(out) & 7) || (out_stride % 4)) return VT_ERR_INVALID;   // rows are stored 8 bytes at a time
+  }
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_stride % 8) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return VT_ERR_INVALID;
   if (q_stride < static_cast<int64_t>(h) * d || out_stride < static_cast<int64_t>(h) * d) return VT_ERR_INVALID;
@@ -216,6 +254,20 @@ static int decode_attn_impl(void *out, int64_t out_stride, const void *q, int64_
   p.out = out; p.out_stride = out_stride; p.q = q; p.q_stride = q_stride;
   p.k_table = k_table; p.v_table = v_table; p.slot_ids = slot_ids; p.seq_lens = seq_lens;
   p.batch = batch; p.h = h; p.kvh = kvh; p.scale = scale; p.k_scale = k_scale; p.v_scale = v_scale;
+  if (kv_dtype == VT_KV_INT4 && batch > vt::kFlatMaxBatch) {
+    // the schedule's per-sequence table ends here: the rest of the batch is a call of its own
+    const int n = vt::kFlatMaxBatch;
+    const auto bf16 = [](const void *x, int64_t e) { return x ? static_cast<const uint16_t *>(x) + e : nullptr; };
+    int st = decode_attn_impl(out, out_stride, q, q_stride, k_table, v_table, slot_ids, seq_lens, n, h, kvh, d, max_seq_len,
+                              scale, kv_dtype, k_scale, v_scale, lse, workspace, workspace_bytes, 0, stream, new_key,
+                              new_value, new_key_stride, new_value_stride, byte_off, flags, maps);
+    if (st != VT_OK) return st;
+    return decode_attn_impl(static_cast<uint16_t *>(out) + n * out_stride, out_stride, bf16(q, n * q_stride), q_stride,
+                            k_table, v_table, slot_ids + n, seq_lens + n, batch - n, h, kvh, d, max_seq_len, scale, kv_dtype,
+                            k_scale, v_scale, lse ? lse + static_cast<int64_t>(n) * h : nullptr, workspace, workspace_bytes, 0, stream,
+                            bf16(new_key, n * new_key_stride), bf16(new_value, n * new_value_stride), new_key_stride,
+                            new_value_stride, byte_off ? byte_off + n : nullptr, flags & ~3u, maps);
+  }
   p.lse = lse; p.part_tokens = plan.part_tokens; p.max_parts = plan.max_parts;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool fused = new_key && plan.variant == 2;   // the persistent kernel appends the step's rows itself
@@ -247,6 +299,7 @@ static int decode_attn_impl(void *out, int64_t out_stride, const void *q, int64_
       p.maps = maps;
       return vt::launch_attn_flat_umma(p, s);
     }
+    if (kv_dtype == VT_KV_INT4) return vt::launch_attn_int4(p, s);
     return vt::launch_attn_flat(p, kv_dtype, s);
   }
   vt::carve_workspace(workspace, batch, h, plan.max_parts, &p);

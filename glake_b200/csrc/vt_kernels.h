@@ -50,6 +50,18 @@ struct KvWidenParams {
 };
 int launch_kv_widen(const KvWidenParams &p, int max_seq_len, cudaStream_t stream);
 
+struct KvDequantParams {
+  const uint64_t *k_table, *v_table;  // fp8 or 4-bit ranges
+  const int64_t *slot_ids;
+  const int32_t *seq_lens;            // rows to read per entry
+  const int32_t *row_start;           // first output row of entry i
+  int batch, kvh;
+  const float *k_scale, *v_scale;
+  void *k_out, *v_out;                // bf16 [rows, kvh, 128], contiguous; either may be null
+};
+int launch_kv_dequant(const KvDequantParams &p, int max_seq_len, int kv_dtype, cudaStream_t stream);
+int launch_append_int4(const AppendParams &p, cudaStream_t stream);
+
 struct AttnParams {
   void *out;  int64_t out_stride;     // bf16, elements per batch row
   const void *q; int64_t q_stride;
@@ -76,6 +88,10 @@ struct AttnParams {
   const void *maps;                   // tcgen05 engine only: device table [slot][K, V] of 128-byte TMA tensor maps
   int overlap;                        // launched as a programmatic dependent of the previous kernel on the stream:
                                       // 1 = its inputs are ready already, 2 = wait for that kernel before reading q / new rows
+  // weight accumulation: the engines also write every logit and, per (entry, q head), the softmax statistics
+  float *logits;                      // [batch, kvh, logit_rows, h / kvh], log2 domain; nullptr = off
+  int logit_rows;
+  float *ml;                          // [batch, h, 2]: (maximum in the log2 domain, sum); with logits
 };
 
 constexpr int kFlatMaxBatch = 1024;   // prefix table of the flat schedule lives in shared memory
@@ -125,6 +141,7 @@ int launch_attn_reduce(const AttnParams &p, int kv_dtype, cudaStream_t stream);
 // fp8 cache on tcgen05 (same schedule and scratch as the flat kernel); needs p.maps from encode_decode_maps_f8
 int launch_attn_flat_umma(const AttnParams &p, cudaStream_t stream);
 bool attn_flat_umma_supports(int batch, int h, int kvh, int kv_dtype);
+int launch_attn_int4(const AttnParams &p, cudaStream_t stream);
 int encode_decode_maps_f8(const uint64_t *k_bases, const uint64_t *v_bases, int n_slots, int kvh, uint64_t max_tokens,
                           void *host_maps);
 

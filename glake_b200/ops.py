@@ -10,7 +10,7 @@ from ctypes import byref, c_size_t, c_void_p
 
 import torch
 
-from ._lib import VT_KV_BF16, VT_KV_FP8_E4M3, check, lib
+from ._lib import VT_KV_BF16, VT_KV_FP8_E4M3, VT_KV_INT4, check, lib
 
 _workspaces = {}
 
@@ -34,7 +34,16 @@ def _kv_dtype(kv_cache_dtype):
         return VT_KV_BF16
     if kv_cache_dtype in ("fp8", "fp8_e4m3"):
         return VT_KV_FP8_E4M3
-    raise RuntimeError(f"unsupported kv_cache_dtype {kv_cache_dtype!r} (bf16 and fp8_e4m3 only)")
+    if kv_cache_dtype == "int4":
+        return VT_KV_INT4
+    raise RuntimeError(f"unsupported kv_cache_dtype {kv_cache_dtype!r} (bf16, fp8_e4m3 and int4 only)")
+
+
+def kv_row_bytes(num_kv_heads, head_size, kv_cache_dtype="auto"):
+    """Bytes of one token's K (or V) row of all kv heads in a range of this cache type."""
+    n = c_size_t()
+    check(lib.vt_kv_row_bytes(num_kv_heads, head_size, _kv_dtype(kv_cache_dtype), byref(n)), "vt_kv_row_bytes")
+    return n.value
 
 
 def new_workspace(device, batch, num_heads, head_size, max_seq_len):
@@ -67,7 +76,8 @@ def reshape_and_cache(key, value, key_cache, value_cache, slot_m, slot_mapping, 
     ``value_cache`` are int64 device tensors of base addresses indexed by slot id,
     ``slot_m`` the per-entry destination byte offsets, ``slot_mapping`` the slot
     ids, ``max_seq_len`` 1 for decode.  The keyword arguments add the fp8 e4m3
-    cache with per-kv-head scales (float32 device tensors of num_kv_heads)."""
+    cache and the 4-bit cache (``"int4"``: an e4m3 scale per 32 dims, see vt_append) with
+    per-kv-head scales (float32 device tensors of num_kv_heads, for both from :func:`kv_scales`)."""
     _require_cuda(key, value, key_cache, value_cache, slot_m, slot_mapping)
     if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
         raise RuntimeError("reshape_and_cache: key/value must be bfloat16")
@@ -190,7 +200,7 @@ def paged_attention_v1(out, query, key_cache, value_cache, num_kv_heads, scale, 
     if query.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         raise RuntimeError("paged_attention_v1: bf16 only")
     kvd = _kv_dtype(kv_cache_dtype)
-    if kvd == VT_KV_FP8_E4M3 and k_scale is None:
+    if kvd != VT_KV_BF16 and k_scale is None:
         k_scale = torch.full((num_kv_heads,), float(kv_scale), dtype=torch.float32, device=query.device)
         v_scale = k_scale
     _decode(out, query, key_cache, value_cache, num_kv_heads, scale, seq_lens, max_seq_len, slot_mapping, kvd,
@@ -286,8 +296,8 @@ def decode_step(out, query, key, value, key_cache, value_cache, slot_m, slot_map
 
 def step_is_fused(kv_cache_dtype):
     """Whether decode_step on the persistent schedule is ONE launch for this cache type: the
-    attention kernel appends the new rows itself (bf16: copied, fp8: quantised on the way)."""
-    return _kv_dtype(kv_cache_dtype) in (VT_KV_BF16, VT_KV_FP8_E4M3)
+    attention kernel appends the new rows itself (bf16: copied, fp8 and int4: quantised on the way)."""
+    return _kv_dtype(kv_cache_dtype) in (VT_KV_BF16, VT_KV_FP8_E4M3, VT_KV_INT4)
 
 
 def prefill_tma_supported(num_kv_heads):
@@ -334,8 +344,8 @@ def decode_maps(k_bases, v_bases, num_kv_heads, head_size, max_tokens, device, k
 
 
 def widen_fp8_ranges(key_cache, value_cache, num_kv_heads, head_size, slot_mapping, seq_lens, k_scale, v_scale,
-                     pad_rows=64):
-    """Dense bf16 copies of the slots' fp8 rows for the prompt kernels: returns
+                     pad_rows=64, kv_cache_dtype="fp8_e4m3"):
+    """Dense bf16 copies of the slots' fp8 (or, with ``kv_cache_dtype="int4"``, 4-bit) rows for the prompt kernels: returns
     (k_bases, v_bases, holder) where ``k_bases`` / ``v_bases`` are int64 device tensors
     of one scratch range address per batch entry (usable as pointer tables with slot ids
     0..B-1) and ``holder`` keeps the scratch alive.  Every entry's range is padded to a
@@ -353,11 +363,40 @@ def widen_fp8_ranges(key_cache, value_cache, num_kv_heads, head_size, slot_mappi
         acc += n
     kb = torch.tensor([buf[0].data_ptr() + s * row * 2 for s in starts], dtype=torch.int64, device=dev)
     vb = torch.tensor([buf[1].data_ptr() + s * row * 2 for s in starts], dtype=torch.int64, device=dev)
+    if _kv_dtype(kv_cache_dtype) == VT_KV_INT4:
+        dequantize_ranges(buf[0].view(-1, num_kv_heads, head_size), buf[1].view(-1, num_kv_heads, head_size), key_cache,
+                          value_cache, num_kv_heads, slot_mapping, seq_lens,
+                          torch.tensor(starts, dtype=torch.int32, device=dev), max(lens) if lens else 0, kv_cache_dtype,
+                          k_scale, v_scale)
+        return kb, vb, (buf, padded)
     with torch.cuda.device(dev):
         check(lib.vt_kv_widen(c_void_p(int(key_cache)), c_void_p(int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens),
                               len(lens), num_kv_heads, head_size, max(lens) if lens else 0, _ptr(k_scale), _ptr(v_scale),
                               _ptr(kb), _ptr(vb), _stream()), "vt_kv_widen")
     return kb, vb, (buf, padded)
+
+
+def dequantize_ranges(key_out, value_out, key_cache, value_cache, num_kv_heads, slot_mapping, seq_lens, row_start,
+                      max_seq_len, kv_cache_dtype="fp8_e4m3", k_scale=None, v_scale=None):
+    """Reads a quantised cache back: rows ``0 .. seq_lens[i]`` of entry i's ranges as bf16 rows
+    ``row_start[i] ..`` of ``key_out`` / ``value_out`` ([rows, kv_heads, head_size], contiguous; one
+    of the two may be None).  ``key_cache`` / ``value_cache`` are pointer-table addresses (ints),
+    ``seq_lens`` / ``row_start`` int32, ``max_seq_len`` a host bound of ``seq_lens``."""
+    outs = [t for t in (key_out, value_out) if t is not None]
+    if not outs:
+        raise RuntimeError("dequantize_ranges: no output")
+    _require_cuda(*outs, slot_mapping, seq_lens, row_start, k_scale, v_scale)
+    head_size = outs[0].shape[-1]
+    for t in outs:
+        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.numel() % (num_kv_heads * head_size):
+            raise RuntimeError("dequantize_ranges: outputs must be contiguous bfloat16 [rows, kv_heads, head_size]")
+    if slot_mapping.dtype != torch.int64 or seq_lens.dtype != torch.int32 or row_start.dtype != torch.int32:
+        raise RuntimeError("dequantize_ranges: slot_mapping must be int64, seq_lens and row_start int32")
+    with torch.cuda.device(outs[0].device):
+        check(lib.vt_kv_dequant(c_void_p(int(key_cache)), c_void_p(int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens),
+                                _ptr(row_start), slot_mapping.numel(), num_kv_heads, head_size, int(max_seq_len),
+                                _kv_dtype(kv_cache_dtype), _ptr(k_scale), _ptr(v_scale), _ptr(key_out), _ptr(value_out),
+                                _stream()), "vt_kv_dequant")
 
 
 def prefill_attention(out, query, key_cache, value_cache, num_kv_heads, scale, slot_mapping, seq_lens, q_lens,
@@ -367,7 +406,7 @@ def prefill_attention(out, query, key_cache, value_cache, num_kv_heads, scale, s
     ``key_cache`` / ``value_cache`` the pointer-table addresses (ints), ``seq_lens``
     the contexts including the new tokens, ``q_lens`` / ``q_start`` int32 per entry.
     With ``maps`` (from :func:`prefill_maps`) K/V tiles are fetched by TMA tensor copies.
-    An fp8 e4m3 cache (``kv_cache_dtype``, per-kv-head ``k_scale`` / ``v_scale``) is first
+    An fp8 e4m3 or int4 cache (``kv_cache_dtype``, per-kv-head ``k_scale`` / ``v_scale``) is first
     widened into bf16 scratch ranges (:func:`widen_fp8_ranges`), over which the same
     kernels run, with tensor maps of the scratch where the head count allows."""
     _require_cuda(out, query, slot_mapping, seq_lens, q_lens, q_start, maps)
@@ -375,11 +414,11 @@ def prefill_attention(out, query, key_cache, value_cache, num_kv_heads, scale, s
         raise RuntimeError("prefill_attention: bf16 only")
     n, num_heads, head_size = query.shape
     holder = None
-    if _kv_dtype(kv_cache_dtype) == VT_KV_FP8_E4M3:
+    if _kv_dtype(kv_cache_dtype) != VT_KV_BF16:
         if k_scale is None or v_scale is None:
-            raise RuntimeError("prefill_attention: an fp8 cache needs k_scale and v_scale")
+            raise RuntimeError(f"prefill_attention: an {kv_cache_dtype} cache needs k_scale and v_scale")
         kb, vb, holder = widen_fp8_ranges(key_cache, value_cache, num_kv_heads, head_size, slot_mapping, seq_lens,
-                                          k_scale, v_scale)
+                                          k_scale, v_scale, kv_cache_dtype=kv_cache_dtype)
         batch = slot_mapping.numel()
         key_cache, value_cache = kb.data_ptr(), vb.data_ptr()
         slot_mapping = torch.arange(batch, dtype=torch.int64, device=query.device)

@@ -55,7 +55,8 @@ const char *vt_version(void);
 /* ---- KV element types -------------------------------------------------- */
 enum {
   VT_KV_BF16 = 0,     /* 2-byte cache elements, bit-exact copy of the inputs      */
-  VT_KV_FP8_E4M3 = 1  /* 1-byte e4m3 (max 448), stored = sat(x / scale[kv_head]) */
+  VT_KV_FP8_E4M3 = 1, /* 1-byte e4m3 (max 448), stored = sat(x / scale[kv_head]) */
+  VT_KV_INT4 = 2      /* 4-bit elements with a group scale per 32 of them: see vt_append  */
 };
 
 /* ---- allocator --------------------------------------------------------- */
@@ -182,7 +183,14 @@ int vt_pool_write(vt_pool *pool, uint64_t dst_dptr, const void *src_host, size_t
  *                 VT_KV_FP8_E4M3: byte = sat_e4m3(x / scale[kv_head]),
  *                 row = kvh*d bytes, k_scale/v_scale device float[kvh]
  *                 (fp8 storage has no counterpart on the reference's vTensor
- *                 path; arithmetic follows csrc/quantization/fp8/nvidia/quant_utils.cuh:467-479)
+ *                 path; arithmetic follows csrc/quantization/fp8/nvidia/quant_utils.cuh:467-479);
+ *                 VT_KV_INT4: per 32 dims of a head s = e4m3(amax / (7 scale[kv_head])),
+ *                 saturating at 448, and q = clamp(round(x / (s scale[kv_head])), -7, 7), ties to
+ *                 even; NaN is stored as 0 and infinities saturate; k_scale/v_scale as for fp8;
+ *                 row = vt_kv_row_bytes: every unit of U kv heads is U x 64 bytes, dim
+ *                 32 G + 4 r + j in byte 8 r + 2 G + j / 2 (low nibble for even j) as q + 8, then
+ *                 U x 4 bytes with the e4m3 scales of the groups G = 0..3, then padding to 16 bytes
+ *                 (not written); no counterpart in the reference
  * d must be 128. */
 int vt_append(const void *key, const void *value, int64_t key_stride, int64_t value_stride,
               const uint64_t *k_table, const uint64_t *v_table, const int64_t *byte_off,
@@ -209,6 +217,21 @@ int vt_kv_scales(const void *x, int64_t stride, int n_tokens, int kvh, int d, fl
 int vt_kv_widen(const uint64_t *k_table, const uint64_t *v_table, const int64_t *slot_ids, const int32_t *seq_lens,
                 int batch, int kvh, int d, int max_seq_len, const float *k_scale, const float *v_scale,
                 const uint64_t *k_out, const uint64_t *v_out, void *stream);
+
+/* Bytes of one token's row of K (or of V) of all kv heads: kvh * d * 2 (bf16), kvh * d (fp8);
+ * 4-bit: kvh / U units of 64 U + round_up(4 U, 16) bytes, U the largest of 8, 4, 2, 1 that
+ * divides kvh. */
+int vt_kv_row_bytes(int kvh, int d, int kv_dtype, size_t *bytes);
+
+/* Reads a quantised cache back: rows [0, seq_lens[i]) of entry i's K and V ranges become bf16
+ * rows row_start[i], row_start[i] + 1, ... of k_out / v_out ([rows, kvh, d], contiguous,
+ * 16-byte aligned; either may be NULL to skip it).  max_seq_len bounds seq_lens on the host.
+ * kv_dtype VT_KV_FP8_E4M3 or VT_KV_INT4; element = stored value * scale[kv_head], rounded once
+ * to bf16.  Nothing synchronises. */
+int vt_kv_dequant(const uint64_t *k_table, const uint64_t *v_table, const int64_t *slot_ids,
+                  const int32_t *seq_lens, const int32_t *row_start, int batch, int kvh, int d,
+                  int max_seq_len, int kv_dtype, const float *k_scale, const float *v_scale, void *k_out,
+                  void *v_out, void *stream);
 
 /* ---- decode attention -------------------------------------------------- */
 /* Scratch bytes vt_decode_attn needs for this problem size (max_seq_len is an

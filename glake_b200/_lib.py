@@ -104,6 +104,16 @@ def _load():
                                    c_int, c_int, c_int, c_float, c_int, vp, vp, vp, vp, sz, ctypes.c_uint, vp]),
         "vt_decode_step_tma": (c_int, [vp, c_int64, vp, c_int64, vp, vp, c_int64, c_int64, vp, vp, vp, vp, vp, c_int, c_int,
                                        c_int, c_int, c_int, c_float, c_int, vp, vp, vp, vp, sz, ctypes.c_uint, vp, vp]),
+        "vt_decode_scored_workspace_bytes": (c_int, [c_int, c_int, c_int, c_int, POINTER(sz)]),
+        "vt_decode_step_scored": (c_int, [vp, c_int64, vp, c_int64, vp, vp, c_int64, c_int64, vp, vp, vp, vp, vp, c_int, c_int,
+                                          c_int, c_int, c_int, c_float, c_int, vp, vp, vp, vp, c_int64, c_int64, c_int, vp,
+                                          sz, vp]),
+        "vt_prompt_scores_workspace_bytes": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, POINTER(sz)]),
+        "vt_prompt_scores": (c_int, [vp, c_int64, c_int64, c_int, vp, c_int64, vp, vp, vp, vp, vp, vp, c_int, c_int, c_int,
+                                     c_int, c_int, c_int, c_float, vp, sz, vp]),
+        "vt_evict_workspace_bytes": (c_int, [c_int, c_int, c_int, c_int, POINTER(sz)]),
+        "vt_evict_rows": (c_int, [vp, vp, c_int64, c_int64, c_int, vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_int, c_int,
+                                  c_int, c_int, vp, vp, sz, vp]),
         "vt_decode_maps_encode": (c_int, [vp, vp, c_int, c_int, c_int, c_int, c_uint64, vp]),
         "vt_prefill_attn": (c_int, [vp, c_int64, vp, c_int64, vp, vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_int,
                                     c_float, c_int, vp, vp]),

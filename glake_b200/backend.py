@@ -109,6 +109,40 @@ class VTensorCacheEngine:
                 self.num_kv_heads, self.head_size, self.max_context_size // self.token_size, self.device)
         return self._decode_maps[layer]
 
+    def new_scores(self, max_rows=None):
+        """One zero-filled float32 tensor ``[slots, kv_heads, rows]`` per layer for the accumulated attention
+        weights (``scores=`` of :meth:`VTensorAttentionImpl.forward`).  A slot's rows must be zero when a new
+        sequence takes it over: ``scores[layer][slot].zero_()``."""
+        rows = max_rows or self.max_context_size // self.token_size
+        return [torch.zeros(len(self.vmm_kvcache_segment), self.num_kv_heads, rows, dtype=torch.float32, device=self.device)
+                for _ in range(self.num_layers)]
+
+    def evict(self, scores, slots, seq_lens, budget, sink=0, recent=0, release=True):
+        """Cuts the sequences in ``slots`` (distinct) to at most ``budget`` rows in every layer by the accumulated
+        weights (:func:`ops.evict_rows`), shortens them in the allocator and returns their new lengths and the kept
+        row numbers per layer.  ``release`` waits for the kernels and unmaps the chunks behind the kept rows; without
+        it they stay mapped for the rows to come."""
+        if len(set(slots)) != len(slots):
+            raise RuntimeError("evict: the slots of a call must be distinct")
+        ids = torch.tensor(list(slots), dtype=torch.int64, device=self.device)
+        lens = torch.tensor(list(seq_lens), dtype=torch.int32, device=self.device)
+        kept = []
+        for layer in range(self.num_layers):
+            kc, vc = self.gpu_cache[layer]
+            kept.append(ops.evict_rows(scores[layer], kc.vmm_ptr, vc.vmm_ptr, self.num_kv_heads, ids, lens,
+                                       max(seq_lens, default=0), budget, sink, recent, self.cache_dtype,
+                                       head_size=self.head_size))
+        new_lens = [min(int(n), int(budget)) for n in seq_lens]
+        if release:
+            torch.cuda.synchronize(self.device)   # nothing may read the rows that are about to be unmapped
+        for slot, n in zip(slots, new_lens):
+            seg = self.vmm_kvcache_segment[slot]
+            if release:
+                seg.trim(n * self.token_size)
+            else:
+                seg.set_used_size(n * self.token_size)
+        return new_lens, kept
+
     def close(self):
         self._prefill_maps = {}
         self._decode_maps = {}
@@ -215,18 +249,22 @@ class VTensorAttentionImpl:
             raise ValueError("head size 128 only")
 
     def forward(self, query, key, value, key_cache: KV_cache, value_cache: KV_cache, attn_metadata: VTensorMetadata,
-                kv_scale: float = 1.0, k_scale=None, v_scale=None, prefill_maps=None, decode_maps=None):
+                kv_scale: float = 1.0, k_scale=None, v_scale=None, prefill_maps=None, decode_maps=None, scores=None,
+                score_window=32):
         """query ``[tokens, H*D]``, key/value ``[tokens, KVH*D]`` -> ``[tokens, H*D]``.
         ``prefill_maps``: the layer's tensor-map table (``VTensorCacheEngine.prefill_maps``),
         used by the prompt branch when given; ``decode_maps``: the one of an fp8 cache for the
         decode branch (``VTensorCacheEngine.decode_maps``: the tcgen05 kernel).  ``k_scale`` / ``v_scale``: the layer's per-kv-head
-        scales of an fp8 cache (``ops.kv_scales`` of the first prompt's rows, then frozen)."""
+        scales of an fp8 or int4 cache (``ops.kv_scales`` of the first prompt's rows, then frozen).
+        ``scores`` (the layer's tensor of ``VTensorCacheEngine.new_scores``) receives the attention
+        weights of this call's queries: of the token in a decode step, of the last ``score_window``
+        tokens of a prompt."""
         with nvtx_range("vtensor attention: prompt" if attn_metadata.num_prefills > 0 else "vtensor attention: decode"):
             return self._forward(query, key, value, key_cache, value_cache, attn_metadata, k_scale, v_scale,
-                                 prefill_maps, decode_maps)
+                                 prefill_maps, decode_maps, scores, score_window)
 
     def _forward(self, query, key, value, key_cache, value_cache, attn_metadata, k_scale, v_scale, prefill_maps,
-                 decode_maps=None):
+                 decode_maps=None, scores=None, score_window=32):
         query = query.view(-1, self.num_heads, self.head_size)
         key = key.view(-1, self.num_kv_heads, self.head_size)
         value = value.view(-1, self.num_kv_heads, self.head_size)
@@ -247,13 +285,17 @@ class VTensorAttentionImpl:
                                   m.slot_mapping, m.seq_lens_tensor, m.query_lens_tensor, m.cache_seq_lens,
                                   m.max_query_len, maps=prefill_maps, kv_cache_dtype=self.kv_cache_dtype,
                                   k_scale=k_scale, v_scale=v_scale)
+            if scores is not None:
+                ops.prompt_scores(scores, query, key_cache.vmm_ptr, self.num_kv_heads, self.scale, m.slot_mapping,
+                                  m.seq_lens_tensor, m.query_lens_tensor, m.cache_seq_lens, m.max_seq_len, score_window,
+                                  self.kv_cache_dtype, k_scale)
             return output.view(-1, self.num_heads * self.head_size)
         # append + attention of the layer as one fused step (one kernel launch for a
         # bf16 cache); equivalent to ops.reshape_and_cache followed by ops.fwd_kvcache
         output = torch.empty_like(query)
         ops.decode_step(output, query, key, value, key_cache.vmm_ptr, value_cache.vmm_ptr, m.slot_m, m.slot_mapping,
                         m.seq_lens_tensor, m.max_seq_len, self.num_kv_heads, self.scale, self.kv_cache_dtype,
-                        k_scale, v_scale, maps=decode_maps)
+                        k_scale, v_scale, maps=decode_maps, scores=scores)
         return output.view(-1, self.num_heads * self.head_size)
 
 

@@ -142,6 +142,22 @@ class ChunkSpaceManager:
             self.block_tables[seq.slot] += 2
         return True
 
+    # -- eviction of rows -----------------------------------------------
+    def evicted(self, seq: SequenceChunks, n_tokens: int) -> None:
+        """The sequence was cut to ``n_tokens`` rows (``VTensorCacheEngine.evict``): its logical
+        reservation starts over at that length, headroom included, and the chunks behind it
+        go back to the budget (never those of a pre-cached prefix, never more than the slot holds)."""
+        held = self.block_tables[seq.slot]
+        seq.reserve_size = seq.free_size = seq.logical_block_num = 0
+        seq.append_tokens(n_tokens)
+        floor = 2 * self.cache_token if held >= 2 * self.cache_token else 0
+        keep = min(held, max(seq.logical_block_num, floor))
+        seq.reserve_size = min(seq.reserve_size, keep // 2 * PHY_GRAN)
+        seq.logical_block_num = min(seq.logical_block_num, keep)
+        seq.free_size = max(0, min(seq.free_size, seq.reserve_size - seq.token_size * n_tokens))
+        self.num_free += held - keep
+        self.block_tables[seq.slot] = keep
+
     # -- end of life ---------------------------------------------------
     def free(self, seq: SequenceChunks) -> int:
         """Finished sequence: keep the pre-cached prefix of the slot if it holds at
@@ -180,6 +196,11 @@ def apply_allocate(seq: SequenceChunks, segment) -> None:
     the kernels reach the new chunk: the 2 x layers driver calls of a growth (tens of
     milliseconds for a deep model) never sit on a step's critical path."""
     segment.ensure_mapped(seq.reserve_size)
+
+
+def apply_evicted(seq: SequenceChunks, n_tokens: int, segment) -> None:
+    """Unmap what ``ChunkSpaceManager.evicted`` gave back (after the evicting kernels have finished)."""
+    segment.trim(n_tokens * seq.token_size, seq.reserve_size)
 
 
 def apply_extend(extend_seq_list: List[int], segments, token_bytes: int) -> None:

@@ -82,7 +82,8 @@ int sm_count() {
 // W = per-warp engine (WarpAttn: bf16 cache, 4 consumer warps; WarpAttnF8: fp8 e4m3
 // cache, 8 consumer warps), NB = 8-head blocks per kv head, HS = kv heads per CTA,
 // R = consecutive tokens per 1 KiB bulk copy; HS * R = consumer warps.
-template <template <int> class W, int NB, int HS, int R>
+// LOG: the weight-accumulating form, which also writes every logit and the softmax statistics (AttnParams::logits).
+template <template <int> class W, int NB, int HS, int R, bool LOG>
 __global__ void __launch_bounds__((W<NB>::kWarps + 1) * 32, NB == 1 ? FlatCfg<W, NB>::kCtasPerSm : 1)
 attn_flat_kernel(AttnParams p) {
   constexpr int kCWarps = W<NB>::kWarps;
@@ -118,7 +119,8 @@ attn_flat_kernel(AttnParams p) {
   }
   // tiles per sequence, then an exclusive prefix (batch is small: one warp scans it)
   for (int i = threadIdx.x; i < p.batch; i += kThreads) {
-    const int len = max(p.seq_lens[i], 0);
+    int len = max(p.seq_lens[i], 0);
+    if constexpr (LOG) len = min(len, p.logit_rows);   // the logits have room for no more
     lens[i] = len;
     prefix[i + 1] = len > 0 ? ((len + TILE_TOK - 1) / TILE_TOK + kBoundaryCost) * slabs : 0;
     if (cache_bases) {   // resolve slot -> range base once, off the producer's critical path
@@ -292,7 +294,13 @@ attn_flat_kernel(AttnParams p) {
           __syncwarp();
         }
       }
-      if (tok0 < seq_len) st.tile(ring0 + s * kStageB, smem + s * kStageB, k_off, v_off, row_off, n_rows, sl2, lane);
+      if constexpr (LOG) {
+        float *lg = p.logits + ((static_cast<size_t>(pc.b) * p.kvh + kv_head) * p.logit_rows + tok0) * g;
+        if (tok0 < seq_len)
+          st.template tile<true>(ring0 + s * kStageB, smem + s * kStageB, k_off, v_off, row_off, n_rows, sl2, lane, lg, R * g, g);
+      } else {
+        if (tok0 < seq_len) st.tile(ring0 + s * kStageB, smem + s * kStageB, k_off, v_off, row_off, n_rows, sl2, lane);
+      }
       // this warp's own stores into the stage (zeroed rows of a ragged tile, a quantised new row)
       // must be ordered before the copy engine refills the stage
       if (n_rows < 16 || (kFp8 && newest_here)) fence_proxy_async();
@@ -393,14 +401,14 @@ attn_flat_kernel(AttnParams p) {
   if (failed && lane == 0) atomicExch(p.status, kKernelErrMagic);
 }
 
-template <template <int> class W, int NB, int HS, int R>
-int launch(const AttnParams &p_in, cudaStream_t stream) {
+template <template <int> class W, int NB, int HS, int R, bool LOG>
+int launch_as(const AttnParams &p_in, cudaStream_t stream) {
   constexpr int kThreads = (W<NB>::kWarps + 1) * 32;
   AttnParams p = p_in;
   p.n_ctas = FlatCfg<W, NB>::kCtasPerSm * std::min(sm_count(), kFlatSms);
   const int smem = flat_smem_bytes(p.batch, FlatCfg<W, NB>::kStages);
   static SmemOptIn opt_in;
-  if (!opt_in.ensure(attn_flat_kernel<W, NB, HS, R>, smem)) return VT_ERR_CUDA;
+  if (!opt_in.ensure(attn_flat_kernel<W, NB, HS, R, LOG>, smem)) return VT_ERR_CUDA;
   if (p.overlap) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.n_ctas);
@@ -412,10 +420,15 @@ int launch(const AttnParams &p_in, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attn_flat_kernel<W, NB, HS, R>, p) == cudaSuccess ? VT_OK : VT_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, attn_flat_kernel<W, NB, HS, R, LOG>, p) == cudaSuccess ? VT_OK : VT_ERR_CUDA;
   }
-  attn_flat_kernel<W, NB, HS, R><<<p.n_ctas, kThreads, smem, stream>>>(p);
+  attn_flat_kernel<W, NB, HS, R, LOG><<<p.n_ctas, kThreads, smem, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? VT_OK : VT_ERR_CUDA;
+}
+
+template <template <int> class W, int NB, int HS, int R>
+int launch(const AttnParams &p, cudaStream_t stream) {
+  return p.logits ? launch_as<W, NB, HS, R, true>(p, stream) : launch_as<W, NB, HS, R, false>(p, stream);
 }
 
 template <int NB>

@@ -194,13 +194,12 @@ struct WarpAttn4 {
       const float s10 = vb ? s[nb][2] * qmul[nb][0] : -INFINITY, s11 = vb ? s[nb][3] * qmul[nb][1] : -INFINITY;
       if constexpr (LOG) {
         const int head = nb * 8 + 2 * c4;
-        if (head < g) {
+        if (head + 1 < g) {   // head is even, and so is g here: 8-byte aligned
+          if (va) *reinterpret_cast<float2 *>(lg + ta * g + head) = make_float2(s00, s01);
+          if (vb) *reinterpret_cast<float2 *>(lg + tb * g + head) = make_float2(s10, s11);
+        } else if (head < g) {
           if (va) lg[ta * g + head] = s00;
           if (vb) lg[tb * g + head] = s10;
-        }
-        if (head + 1 < g) {
-          if (va) lg[ta * g + head + 1] = s01;
-          if (vb) lg[tb * g + head + 1] = s11;
         }
       }
       float mx0 = fmaxf(s00, s10), mx1 = fmaxf(s01, s11);
@@ -358,7 +357,8 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(A
     mbar_fence_init();
   }
   for (int i = threadIdx.x; i < p.batch; i += kThreads4) {
-    const int len = max(p.seq_lens[i], 0);
+    int len = max(p.seq_lens[i], 0);
+    if constexpr (LOG) len = min(len, p.logit_rows);   // the logits have room for no more
     lens[i] = len;
     prefix[i + 1] = len > 0 ? ((len + TOK - 1) / TOK + kBoundaryCost) * slabs : 0;
     if (cache_bases) {

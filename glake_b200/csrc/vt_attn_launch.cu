@@ -38,6 +38,7 @@ __global__ void __launch_bounds__(kHeadDim) attn_reduce_kernel(AttnParams p) {
   const float vs = FP8 ? p.v_scale[hq / (p.h / p.kvh)] : 1.0f;
   static_cast<__nv_bfloat16 *>(p.out)[b * p.out_stride + hq * kHeadDim + d] = __float2bfloat16(O / L * vs);
   if (p.lse && d == 0) p.lse[b * p.h + hq] = (M + log2f(L)) * 0.6931471805599453f;
+  if (p.ml && d == 0) *reinterpret_cast<float2 *>(p.ml + 2 * (b * p.h + hq)) = make_float2(M, L);
 }
 
 }  // namespace
@@ -213,8 +214,8 @@ int vt_kv_dequant(const uint64_t *k_table, const uint64_t *v_table, const int64_
   if (!slot_ids || !seq_lens || !row_start || (!k_out && !v_out)) return VT_ERR_INVALID;
   if ((k_out && (!k_table || !k_scale)) || (v_out && (!v_table || !v_scale))) return VT_ERR_INVALID;
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return VT_ERR_INVALID;
-  vt::KvDequantParams p{k_table, v_table, slot_ids, seq_lens, row_start, batch, kvh, k_scale, v_scale, k_out, v_out};
-  return vt::launch_kv_dequant(p, max_seq_len, kv_dtype, static_cast<cudaStream_t>(stream));
+  vt::KvDequantParams p{k_table, v_table, slot_ids, seq_lens, row_start, batch, kvh, max_seq_len, k_scale, v_scale, k_out, v_out};
+  return vt::launch_kv_dequant(p, kv_dtype, static_cast<cudaStream_t>(stream));
 }
 
 int vt_decode_attn_workspace_bytes(int batch, int h, int d, int max_seq_len, size_t *bytes) {
@@ -230,7 +231,8 @@ static int decode_attn_impl(void *out, int64_t out_stride, const void *q, int64_
                    float scale, int kv_dtype, const float *k_scale, const float *v_scale,
                    float *lse, void *workspace, size_t workspace_bytes, int num_splits,
                    void *stream, const void *new_key, const void *new_value, int64_t new_key_stride,
-                   int64_t new_value_stride, const int64_t *byte_off, unsigned flags, const void *maps = nullptr) {
+                   int64_t new_value_stride, const int64_t *byte_off, unsigned flags, const void *maps = nullptr,
+                   float *logits = nullptr, int logit_rows = 0, float *ml = nullptr) {
   if (batch < 0 || h <= 0 || kvh <= 0 || max_seq_len < 0 || num_splits < 0) return VT_ERR_INVALID;
   if (batch == 0) return VT_OK;
   if (!out || !q || !k_table || !v_table || !slot_ids || !seq_lens || !workspace) return VT_ERR_INVALID;
@@ -249,8 +251,15 @@ static int decode_attn_impl(void *out, int64_t out_stride, const void *q, int64_
   if (q_stride < static_cast<int64_t>(h) * d || out_stride < static_cast<int64_t>(h) * d) return VT_ERR_INVALID;
   vt::AttnPlan plan;
   vt::plan_attn(batch, h, kvh, std::max(max_seq_len, 1), kv_dtype, num_splits, &plan);
+  if (logits && plan.variant == 1) {
+    // the split-K kernel has no accumulating form: the persistent one, or SIMT for the shapes that one does not take
+    plan.variant = vt::attn_flat_supports(batch, h, kvh, kv_dtype) ? 2 : 0;
+    plan.ws_bytes = plan.variant == 2 ? vt::flat_workspace_bytes(batch, h, kvh, kv_dtype)
+                                      : vt::attn_workspace_bytes(batch, h, plan.max_parts);
+  }
   if (plan.ws_bytes > workspace_bytes) return VT_ERR_INVALID;
   vt::AttnParams p{};
+  p.logits = logits; p.logit_rows = logit_rows; p.ml = ml;
   p.out = out; p.out_stride = out_stride; p.q = q; p.q_stride = q_stride;
   p.k_table = k_table; p.v_table = v_table; p.slot_ids = slot_ids; p.seq_lens = seq_lens;
   p.batch = batch; p.h = h; p.kvh = kvh; p.scale = scale; p.k_scale = k_scale; p.v_scale = v_scale;
@@ -431,6 +440,145 @@ int vt_decode_step_tma(void *out, int64_t out_stride, const void *q, int64_t q_s
   return decode_attn_impl(out, out_stride, q, q_stride, k_table, v_table, slot_ids, seq_lens, batch, h, kvh, d,
                           max_seq_len, scale, kv_dtype, k_scale, v_scale, lse, workspace, workspace_bytes, 0, stream,
                           key, value, key_stride, value_stride, byte_off, flags, maps);
+}
+
+static size_t scored_ml_bytes(int batch, int h) { return (static_cast<size_t>(batch) * h * 8 + 255) / 256 * 256; }
+
+int vt_decode_scored_workspace_bytes(int batch, int h, int d, int max_seq_len, size_t *bytes) {
+  if (!bytes || batch < 0 || h <= 0 || max_seq_len < 0) return VT_ERR_INVALID;
+  if (d != vt::kHeadDim) return VT_ERR_UNSUPPORTED;
+  const int n = std::min(std::max(batch, 1), vt::kFlatMaxBatch), len = std::max(max_seq_len, 1);   // larger batches run in parts
+  *bytes = (vt::attn_workspace_bound(n, h, len) + 255) / 256 * 256 + scored_ml_bytes(n, h) +
+           static_cast<size_t>(n) * h * len * sizeof(float);
+  return VT_OK;
+}
+
+int vt_decode_step_scored(void *out, int64_t out_stride, const void *q, int64_t q_stride, const void *key,
+                          const void *value, int64_t key_stride, int64_t value_stride, const int64_t *byte_off,
+                          const uint64_t *k_table, const uint64_t *v_table, const int64_t *slot_ids,
+                          const int32_t *seq_lens, int batch, int h, int kvh, int d, int max_seq_len, float scale,
+                          int kv_dtype, const float *k_scale, const float *v_scale, float *lse, float *scores,
+                          int64_t score_slot_stride, int64_t score_head_stride, int score_rows, void *workspace,
+                          size_t workspace_bytes, void *stream) {
+  if (batch < 0 || h <= 0 || kvh <= 0 || max_seq_len < 0 || score_rows < 0) return VT_ERR_INVALID;
+  if (batch == 0) return VT_OK;
+  if (d != vt::kHeadDim || h % kvh != 0) return VT_ERR_UNSUPPORTED;
+  if (!scores || !workspace || !slot_ids || !seq_lens || max_seq_len > score_rows || score_head_stride < score_rows ||
+      score_slot_stride < score_rows)
+    return VT_ERR_INVALID;
+  if (key || value) {
+    if (!key || !value || !byte_off) return VT_ERR_INVALID;
+    if ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15) return VT_ERR_INVALID;
+    if ((key_stride % 8) || (value_stride % 8) || key_stride < static_cast<int64_t>(kvh) * d ||
+        value_stride < static_cast<int64_t>(kvh) * d)
+      return VT_ERR_INVALID;
+  }
+  size_t need = 0;
+  vt_decode_scored_workspace_bytes(batch, h, d, max_seq_len, &need);
+  if (workspace_bytes < need) return VT_ERR_INVALID;
+  const int most = std::min(batch, vt::kFlatMaxBatch);
+  const size_t attn_bytes = (vt::attn_workspace_bound(most, h, std::max(max_seq_len, 1)) + 255) / 256 * 256;
+  float *ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + attn_bytes);
+  float *logits = reinterpret_cast<float *>(static_cast<char *>(workspace) + attn_bytes + scored_ml_bytes(most, h));
+  const auto rows = [](const void *x, int64_t e) { return x ? static_cast<const uint16_t *>(x) + e : nullptr; };
+  for (int b0 = 0; b0 < batch; b0 += most) {
+    const int n = std::min(most, batch - b0);
+    int st = decode_attn_impl(static_cast<uint16_t *>(out) + b0 * out_stride, out_stride, rows(q, b0 * q_stride), q_stride,
+                              k_table, v_table, slot_ids + b0, seq_lens + b0, n, h, kvh, d, max_seq_len, scale, kv_dtype,
+                              k_scale, v_scale, lse ? lse + static_cast<int64_t>(b0) * h : nullptr, workspace, attn_bytes, 0,
+                              stream, rows(key, b0 * key_stride), rows(value, b0 * value_stride), key_stride, value_stride,
+                              byte_off ? byte_off + b0 : nullptr, 0u, nullptr, logits, max_seq_len, ml);
+    if (st != VT_OK) return st;
+    if (max_seq_len == 0) continue;
+    vt::ScoreParams p{logits, max_seq_len, ml, slot_ids + b0, seq_lens + b0, n, kvh, scores, score_slot_stride, score_head_stride};
+    st = vt::launch_accumulate(p, h / kvh, max_seq_len, static_cast<cudaStream_t>(stream));
+    if (st != VT_OK) return st;
+  }
+  return VT_OK;
+}
+
+// Scratch of vt_prompt_scores: the runs' statistics.
+static size_t prompt_scratch(int batch, int kvh, int g, int max_seq_len, int window, int *runs, int *keys) {
+  *keys = vt::prompt_run_keys(batch, kvh, max_seq_len);
+  *runs = std::max(1, (max_seq_len + *keys - 1) / *keys);
+  return static_cast<size_t>(batch) * kvh * *runs * window * g * sizeof(float2);
+}
+
+static int prompt_shape(int batch, int h, int kvh, int d, int max_seq_len, int window) {
+  if (batch < 0 || h <= 0 || kvh <= 0 || max_seq_len < 0 || window < 1) return VT_ERR_INVALID;
+  if (d != vt::kHeadDim || h % kvh != 0) return VT_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(window) * (h / kvh) > 16384) return VT_ERR_UNSUPPORTED;   // rows kept in shared memory
+  return VT_OK;
+}
+
+int vt_prompt_scores_workspace_bytes(int batch, int h, int kvh, int d, int max_seq_len, int window, size_t *bytes) {
+  if (!bytes) return VT_ERR_INVALID;
+  const int st = prompt_shape(batch, h, kvh, d, max_seq_len, window);
+  if (st != VT_OK) return st;
+  int runs, keys;
+  *bytes = std::max<size_t>(prompt_scratch(batch, kvh, h / kvh, max_seq_len, window, &runs, &keys), 256);
+  return VT_OK;
+}
+
+int vt_prompt_scores(float *scores, int64_t score_slot_stride, int64_t score_head_stride, int score_rows, const void *q,
+                     int64_t q_stride, const uint64_t *k_table, const int64_t *slot_ids, const int64_t *range_ids,
+                     const int32_t *seq_lens, const int32_t *q_lens, const int32_t *q_start, int batch, int h, int kvh,
+                     int d, int max_seq_len, int window, float scale, void *workspace, size_t workspace_bytes,
+                     void *stream) {
+  int st = prompt_shape(batch, h, kvh, d, max_seq_len, window);
+  if (st != VT_OK) return st;
+  if (score_rows < 0) return VT_ERR_INVALID;
+  if (batch == 0 || max_seq_len == 0) return VT_OK;
+  if (!scores || !q || !k_table || !slot_ids || !seq_lens || !q_lens || !q_start || !workspace) return VT_ERR_INVALID;
+  if (max_seq_len > score_rows || score_head_stride < score_rows || score_slot_stride < score_rows) return VT_ERR_INVALID;
+  if ((reinterpret_cast<uintptr_t>(q) & 3) || (q_stride % 2) || q_stride < static_cast<int64_t>(h) * d ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return VT_ERR_INVALID;
+  int runs, keys;
+  if (workspace_bytes < prompt_scratch(batch, kvh, h / kvh, max_seq_len, window, &runs, &keys)) return VT_ERR_INVALID;
+  vt::PromptScoreParams p{q, q_stride, k_table, slot_ids, range_ids, seq_lens, q_lens, q_start, batch, h, kvh, max_seq_len,
+                          window, scale, scores, score_slot_stride, score_head_stride, static_cast<float2 *>(workspace),
+                          runs, keys, window * (h / kvh)};
+  return vt::launch_prompt_scores(p, static_cast<cudaStream_t>(stream));
+}
+
+// Scratch of vt_evict_rows: status word, chunk counter, one flag per chunk.
+static size_t evict_scratch(int batch, int kvh, int budget, int kv_dtype, int *chunks) {
+  const int rows = vt::evict_chunk_rows(kv_dtype);
+  *chunks = (budget + rows - 1) / rows;
+  return 512 + static_cast<size_t>(batch) * kvh * *chunks * sizeof(int);
+}
+
+int vt_evict_workspace_bytes(int batch, int kvh, int budget, int kv_dtype, size_t *bytes) {
+  if (!bytes || batch < 0 || kvh <= 0 || budget < 1) return VT_ERR_INVALID;
+  if (kv_dtype != VT_KV_BF16 && kv_dtype != VT_KV_FP8_E4M3 && kv_dtype != VT_KV_INT4) return VT_ERR_UNSUPPORTED;
+  int chunks;
+  *bytes = evict_scratch(batch, kvh, budget, kv_dtype, &chunks);
+  return VT_OK;
+}
+
+int vt_evict_rows(const float *scores, float *scores_out, int64_t score_slot_stride, int64_t score_head_stride,
+                  int score_rows, const uint64_t *k_table, const uint64_t *v_table, const int64_t *slot_ids,
+                  const int32_t *seq_lens, int batch, int kvh, int d, int max_seq_len, int budget, int sink, int recent,
+                  int kv_dtype, int32_t *kept, void *workspace, size_t workspace_bytes, void *stream) {
+  if (batch < 0 || kvh <= 0 || max_seq_len < 0 || score_rows < 0 || budget < 1 || sink < 0 || recent < 0 ||
+      static_cast<int64_t>(sink) + recent > budget)
+    return VT_ERR_INVALID;
+  if (d != vt::kHeadDim) return VT_ERR_UNSUPPORTED;
+  if (kv_dtype != VT_KV_BF16 && kv_dtype != VT_KV_FP8_E4M3 && kv_dtype != VT_KV_INT4) return VT_ERR_UNSUPPORTED;
+  if (batch == 0) return VT_OK;
+  if (!scores || !scores_out || !k_table || !v_table || !slot_ids || !seq_lens || !kept || !workspace) return VT_ERR_INVALID;
+  if (max_seq_len > score_rows || score_head_stride < score_rows || score_slot_stride < score_rows ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return VT_ERR_INVALID;
+  int chunks;
+  if (workspace_bytes < evict_scratch(batch, kvh, budget, kv_dtype, &chunks)) return VT_ERR_INVALID;
+  if (static_cast<int64_t>(batch) * kvh * chunks > 0x7fffffff) return VT_ERR_UNSUPPORTED;
+  char *ws = static_cast<char *>(workspace);
+  vt::EvictParams p{scores, scores_out, score_slot_stride, score_head_stride, k_table, v_table, slot_ids, seq_lens, batch, kvh,
+                    max_seq_len, budget, sink, recent, kept, reinterpret_cast<uint32_t *>(ws), reinterpret_cast<int *>(ws + 256),
+                    reinterpret_cast<int *>(ws + 512), chunks, 0};
+  return vt::launch_evict(p, kv_dtype, static_cast<cudaStream_t>(stream));
 }
 
 int vt_decode_maps_encode(const uint64_t *k_bases, const uint64_t *v_bases, int n_slots, int kvh, int d, int kv_dtype,

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(AttnParams p) {
   const int g_total = p.h / p.kvh, subs = g_total / G;
   const int kv_head = blockIdx.x / subs, sub = blockIdx.x % subs;
   const int part = blockIdx.y, b = blockIdx.z;
-  const int seq_len = p.seq_lens[b];
+  const int seq_len = p.logits ? min(p.seq_lens[b], p.logit_rows) : p.seq_lens[b];
   const int t_begin = part * p.part_tokens;
   if (t_begin >= seq_len && !(part == 0 && seq_len <= 0)) return;
   const int t_end = min(seq_len, t_begin + p.part_tokens);
@@ -172,6 +172,12 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(AttnParams p) {
         sc[g] = v;
       }
     }
+    if (p.logits && valid && j == 0) {   // weight accumulation: qf is pre-scaled, so sc is in the log2 domain already
+      float *lg = p.logits + ((static_cast<size_t>(b) * p.kvh + kv_head) * p.logit_rows + t_begin + tile * kTile + tok) * g_total +
+                  sub * G;
+#pragma unroll
+      for (int g = 0; g < G; ++g) lg[g] = sc[g];
+    }
     if (valid) {
       float pr[G];
 #pragma unroll
@@ -244,6 +250,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(AttnParams p) {
       static_cast<__nv_bfloat16 *>(p.out)[b * p.out_stride + hq * kHeadDim + d] = __float2bfloat16(o);
       if (p.lse && d == 0)
         p.lse[b * p.h + hq] = L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+      if (p.ml && d == 0) *reinterpret_cast<float2 *>(p.ml + 2 * (b * p.h + hq)) = make_float2(M, L);
     } else {
       const size_t idx = (static_cast<size_t>(b) * p.h + hq) * p.max_parts + part;
       p.ws_o[idx * kHeadDim + d] = O;

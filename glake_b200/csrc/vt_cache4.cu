@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kThreads) append_int4_kernel(AppendParams p, i
 template <bool INT4>
 __global__ void __launch_bounds__(kThreads) dequant_kernel(KvDequantParams p, int rows_per_cta) {
   const int i = blockIdx.x;
-  const int n_rows = p.seq_lens[i];
+  const int n_rows = min(p.seq_lens[i], p.max_seq_len);   // the caller made room for no more
   const int t0 = blockIdx.y * rows_per_cta;
   if (t0 >= n_rows) return;
   const int t1 = min(t0 + rows_per_cta, n_rows);
@@ -119,7 +119,8 @@ int launch_append_int4(const AppendParams &p, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? VT_OK : VT_ERR_CUDA;
 }
 
-int launch_kv_dequant(const KvDequantParams &p, int max_seq_len, int kv_dtype, cudaStream_t stream) {
+int launch_kv_dequant(const KvDequantParams &p, int kv_dtype, cudaStream_t stream) {
+  const int max_seq_len = p.max_seq_len;
   if (p.batch == 0 || max_seq_len <= 0) return VT_OK;
   const int rows = std::max(16, (max_seq_len + 65534) / 65535);
   const dim3 grid(p.batch, (max_seq_len + rows - 1) / rows);

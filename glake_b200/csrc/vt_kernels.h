@@ -55,11 +55,11 @@ struct KvDequantParams {
   const int64_t *slot_ids;
   const int32_t *seq_lens;            // rows to read per entry
   const int32_t *row_start;           // first output row of entry i
-  int batch, kvh;
+  int batch, kvh, max_seq_len;
   const float *k_scale, *v_scale;
   void *k_out, *v_out;                // bf16 [rows, kvh, 128], contiguous; either may be null
 };
-int launch_kv_dequant(const KvDequantParams &p, int max_seq_len, int kv_dtype, cudaStream_t stream);
+int launch_kv_dequant(const KvDequantParams &p, int kv_dtype, cudaStream_t stream);
 int launch_append_int4(const AppendParams &p, cudaStream_t stream);
 
 struct AttnParams {
@@ -93,6 +93,54 @@ struct AttnParams {
   int logit_rows;
   float *ml;                          // [batch, h, 2]: (maximum in the log2 domain, sum); with logits
 };
+
+struct ScoreParams {
+  const float *logits;                // as AttnParams
+  int logit_rows;
+  const float *ml;
+  const int64_t *slot_ids;
+  const int32_t *seq_lens;
+  int batch, kvh;
+  float *scores;                      // [slot, kv head, row], innermost contiguous
+  int64_t slot_stride, head_stride;   // elements
+};
+int launch_accumulate(const ScoreParams &p, int g, int max_seq_len, cudaStream_t stream);
+
+struct PromptScoreParams {
+  const void *q; int64_t q_stride;    // bf16 [tokens, h, 128]; stride of a token row in elements
+  const uint64_t *k_table;            // bf16 ranges
+  const int64_t *slot_ids;            // row of scores
+  const int64_t *range_ids;           // index into k_table; nullptr = slot_ids
+  const int32_t *seq_lens, *q_lens, *q_start;
+  int batch, h, kvh, max_seq_len, window;
+  float scale;
+  float *scores;
+  int64_t slot_stride, head_stride;
+  float2 *ml;                         // [batch * kvh, runs, rows]: (maximum in the log2 domain, sum) of a run
+  int runs, run_keys, rows;           // rows = window * (h / kvh)
+};
+int launch_prompt_scores(const PromptScoreParams &p, cudaStream_t stream);
+int prompt_run_keys(int batch, int kvh, int max_seq_len);
+
+struct EvictParams {
+  const float *scores;
+  float *scores_out;
+  int64_t slot_stride, head_stride;
+  const uint64_t *k_table, *v_table;
+  const int64_t *slot_ids;
+  const int32_t *seq_lens;
+  int batch, kvh, max_seq_len;
+  int budget, sink, recent;
+  int32_t *kept;                      // [batch, kvh, budget]
+  uint32_t *status;
+  int *ticket;                        // chunk numbers handed out
+  int *flags;                         // [batch * kvh, chunks]: chunk has read its rows
+  int chunks;                         // of one head
+  int held_rows;                      // weights that fit the selection's shared memory
+};
+constexpr int kMoveRegs = 4;          // 16-byte registers of K, and as many of V, a thread of the move kernel carries
+int evict_chunk_rows(int kv_dtype);
+int launch_evict(const EvictParams &p, int kv_dtype, cudaStream_t stream);
 
 constexpr int kFlatMaxBatch = 1024;   // prefix table of the flat schedule lives in shared memory
 constexpr int kFlatPartRow = 132;     // floats per published piece state row (16-byte aligned)

@@ -51,6 +51,20 @@ constexpr int kPitch = kGroupB + 16;          // pitch between groups
 constexpr int kTileB = kGroupsPerTile * kPitch;
 constexpr int kStageB = 2 * kTileB;
 
+// One fragment's logits (rows r4 and r4 + 8, heads `head` and `head` + 1) to memory, for the weight accumulation.
+__device__ __forceinline__ void store_logits(float *lg, int pitch, int g, int head, int r4, int n_rows, float s00,
+                                             float s01, float s10, float s11) {
+  float *a = lg + r4 * pitch + head, *b = a + 8 * pitch;
+  const bool va = r4 < n_rows, vb = r4 + 8 < n_rows;
+  if (head + 1 < g) {   // head is even, and so is g here: 8-byte aligned
+    if (va) *reinterpret_cast<float2 *>(a) = make_float2(s00, s01);
+    if (vb) *reinterpret_cast<float2 *>(b) = make_float2(s10, s11);
+  } else if (head < g) {
+    if (va) *a = s00;
+    if (vb) *b = s10;
+  }
+}
+
 // Per-warp attention state for one kv head: Q^T fragments of its q heads, the
 // O^T accumulator and the running softmax statistics.
 //   qb[nb][ks][0/1] = Q[head nb*8 + lane/4][16*ks + 2*(lane%4) (+8) .. +1]
@@ -91,8 +105,11 @@ struct WarpAttn {
   // fragment rows are inside the context.  st = shared address of the stage,
   // st_generic the same as a generic pointer; k_off / v_off are the per-lane
   // ldmatrix offsets, row_off the byte offset of the warp's row inside a group.
+  // LOG: the logits (log2 domain) of fragment row i and head j also go to lg[i * lg_pitch + j], j < g.
+  template <bool LOG = false>
   __device__ __forceinline__ void tile(uint32_t st, unsigned char *st_generic, uint32_t k_off, uint32_t v_off,
-                                       uint32_t row_off, int n_rows, float sl2, int lane) {
+                                       uint32_t row_off, int n_rows, float sl2, int lane, float *lg = nullptr,
+                                       int lg_pitch = 0, int g = 0) {
     const int r4 = lane >> 2;
     if (n_rows < 16) {
       // Ragged end: rows past the context hold stale bytes.  Their K only feeds
@@ -123,6 +140,7 @@ struct WarpAttn {
     for (int nb = 0; nb < NB; ++nb) {
       float s00 = v0 ? sacc[nb][0] * sl2 : -INFINITY, s01 = v0 ? sacc[nb][1] * sl2 : -INFINITY;
       float s10 = v1 ? sacc[nb][2] * sl2 : -INFINITY, s11 = v1 ? sacc[nb][3] * sl2 : -INFINITY;
+      if constexpr (LOG) store_logits(lg, lg_pitch, g, nb * 8 + 2 * (lane & 3), r4, n_rows, s00, s01, s10, s11);
       float mx0 = fmaxf(s00, s10), mx1 = fmaxf(s01, s11);
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) {

@@ -75,8 +75,9 @@ struct WarpAttnF8 {
   }
 
   // Arguments as WarpAttn::tile (k_off / v_off unused: offsets follow from lane and row_off).
+  template <bool LOG = false>
   __device__ __forceinline__ void tile(uint32_t, unsigned char *st_generic, uint32_t, uint32_t, uint32_t row_off,
-                                       int n_rows, float sl2, int lane) {
+                                       int n_rows, float sl2, int lane, float *lg = nullptr, int lg_pitch = 0, int g = 0) {
     const int r4 = lane >> 2, c4 = lane & 3;
     if (n_rows < 16) {   // ragged end: clear stale V rows (0 * NaN would poison the accumulators)
       for (int r = n_rows + (lane >> 3); r < 16; r += 4)
@@ -114,6 +115,7 @@ struct WarpAttnF8 {
     for (int nb = 0; nb < NB; ++nb) {
       float s00 = v0 ? sacc[nb][0] * sl2 : -INFINITY, s01 = v0 ? sacc[nb][1] * sl2 : -INFINITY;
       float s10 = v1 ? sacc[nb][2] * sl2 : -INFINITY, s11 = v1 ? sacc[nb][3] * sl2 : -INFINITY;
+      if constexpr (LOG) store_logits(lg, lg_pitch, g, nb * 8 + 2 * c4, r4, n_rows, s00, s01, s10, s11);
       float mx0 = fmaxf(s00, s10), mx1 = fmaxf(s01, s11);
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) {

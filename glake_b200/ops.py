@@ -46,26 +46,41 @@ def kv_row_bytes(num_kv_heads, head_size, kv_cache_dtype="auto"):
     return n.value
 
 
-def new_workspace(device, batch, num_heads, head_size, max_seq_len):
-    """A private, zero-filled scratch buffer for ``decode_step(..., workspace=...)``."""
+def new_workspace(device, batch, num_heads, head_size, max_seq_len, scored=False):
+    """A private, zero-filled scratch buffer for ``decode_step(..., workspace=...)``; ``scored`` adds
+    the room that ``scores=`` needs."""
     need = c_size_t()
-    check(lib.vt_decode_attn_workspace_bytes(batch, num_heads, head_size, max_seq_len, byref(need)),
-          "vt_decode_attn_workspace_bytes")
+    size = lib.vt_decode_scored_workspace_bytes if scored else lib.vt_decode_attn_workspace_bytes
+    check(size(batch, num_heads, head_size, max_seq_len, byref(need)), "new_workspace")
     return torch.zeros(need.value, dtype=torch.uint8, device=device)
 
 
+def _device_index(device):
+    return device.index if device.index is not None else torch.cuda.current_device()
+
+
+def _scratch(device, nbytes):
+    """Scratch cached per device and stream and grown on demand: calls of one stream run back to back, calls of two
+    streams may overlap.  While the stream is being captured the buffer belongs to the capture instead: a graph must
+    not hold the address of a buffer that a later, larger call replaces, nor share one with another graph."""
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(max(nbytes, 1 << 10), dtype=torch.uint8, device=device)
+        key = (_device_index(device), torch.cuda.current_stream().cuda_stream)
+    buf = _workspaces.get(key)
+    if buf is None or buf.numel() < nbytes:
+        buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        _workspaces[key] = buf
+    return buf
+
+
 def attn_workspace(device, batch, num_heads, head_size, max_seq_len):
-    """Scratch for the split-K partials, cached per device and grown on demand.
+    """Scratch for the split-K partials, cached per device and stream and grown on demand.
     One buffer serves every layer because layers run back to back on one stream."""
     need = c_size_t()
     check(lib.vt_decode_attn_workspace_bytes(batch, num_heads, head_size, max_seq_len, byref(need)),
           "vt_decode_attn_workspace_bytes")
-    key = (device.index if device.index is not None else torch.cuda.current_device())
-    buf = _workspaces.get(key)
-    if buf is None or buf.numel() < need.value:
-        buf = torch.zeros(max(need.value, 1 << 20), dtype=torch.uint8, device=device)
-        _workspaces[key] = buf
-    return buf
+    return _scratch(device, need.value)
 
 
 def reshape_and_cache(key, value, key_cache, value_cache, slot_m, slot_mapping, seq_lens, cache_seq_lens,
@@ -163,6 +178,34 @@ def kv_scales(x, num_kv_heads, head_size):
     return out
 
 
+def _check_scores(scores, num_kv_heads, device, what):
+    if scores.dim() != 3 or scores.dtype != torch.float32 or scores.shape[1] != num_kv_heads or scores.stride(2) != 1:
+        raise RuntimeError(f"{what}: scores must be float32 [slots, kv_heads, rows] with contiguous rows")
+    if scores.device != device:
+        raise RuntimeError(f"{what}: scores must be on the device of the other tensors")
+
+
+def _scored(out, query, key, value, slot_m, k_table, v_table, num_kv_heads, scale, seq_lens, max_seq_len, slot_ids,
+            kv_dtype, k_scale, v_scale, lse, scores, workspace=None):
+    batch, num_heads, head_size = query.shape
+    _require_cuda(scores)
+    _check_scores(scores, num_kv_heads, query.device, "scores")
+    ws = workspace
+    if ws is None:
+        need = c_size_t()
+        check(lib.vt_decode_scored_workspace_bytes(batch, num_heads, head_size, int(max_seq_len), byref(need)),
+              "vt_decode_scored_workspace_bytes")
+        ws = _scratch(query.device, need.value)
+    with torch.cuda.device(query.device):
+        check(lib.vt_decode_step_scored(_ptr(out), out.stride(0), _ptr(query), query.stride(0), _ptr(key), _ptr(value),
+                                        key.stride(0) if key is not None else 0,
+                                        value.stride(0) if value is not None else 0, _ptr(slot_m), c_void_p(int(k_table)),
+                                        c_void_p(int(v_table)), _ptr(slot_ids), _ptr(seq_lens), batch, num_heads,
+                                        num_kv_heads, head_size, int(max_seq_len), float(scale), kv_dtype, _ptr(k_scale),
+                                        _ptr(v_scale), _ptr(lse), _ptr(scores), scores.stride(0), scores.stride(1),
+                                        scores.shape[2], _ptr(ws), ws.numel(), _stream()), "vt_decode_step_scored")
+
+
 def _decode(out, query, k_table, v_table, num_kv_heads, scale, seq_lens, max_seq_len, slot_ids, kv_dtype,
             k_scale, v_scale, lse, num_splits, maps=None):
     batch, num_heads, head_size = query.shape
@@ -186,12 +229,15 @@ def _decode(out, query, k_table, v_table, num_kv_heads, scale, seq_lens, max_seq
 
 def paged_attention_v1(out, query, key_cache, value_cache, num_kv_heads, scale, seq_lens, block_size, max_seq_len,
                        alibi_slopes, kv_cache_dtype, kv_scale, slot_mapping, k_scale=None, v_scale=None,
-                       num_splits=0, maps=None):
+                       num_splits=0, maps=None, scores=None):
     """Decode attention with the reference's vTensor signature (csrc/ops.h:6-19):
     ``key_cache`` / ``value_cache`` are the device addresses (ints) of the per-layer
     pointer tables, ``slot_mapping`` the slot ids.  ``block_size`` must be 1 (the
     token-major contiguous layout, vllm/attention/ops/paged_attn.py:105).  ``maps`` (from
-    :func:`decode_maps`, fp8 cache) selects the tcgen05 kernel where the head counts allow."""
+    :func:`decode_maps`, fp8 cache) selects the tcgen05 kernel where the head counts allow.
+    ``scores`` (float32 ``[slots, kv_heads, rows]``) also receives the softmax weight of every cached
+    row, summed over the q heads of its kv head: ``scores[slot, j, t] += ...`` (``maps`` then stay
+    unused, and ``num_splits`` must be 0)."""
     _require_cuda(out, query, seq_lens, slot_mapping, maps)
     if alibi_slopes is not None:
         raise RuntimeError("paged_attention_v1: ALiBi is not supported on the vTensor path")
@@ -203,6 +249,12 @@ def paged_attention_v1(out, query, key_cache, value_cache, num_kv_heads, scale, 
     if kvd != VT_KV_BF16 and k_scale is None:
         k_scale = torch.full((num_kv_heads,), float(kv_scale), dtype=torch.float32, device=query.device)
         v_scale = k_scale
+    if scores is not None:
+        if num_splits:
+            raise RuntimeError("paged_attention_v1: scores needs num_splits = 0")
+        _scored(out, query, None, None, None, key_cache, value_cache, num_kv_heads, scale, seq_lens, max_seq_len,
+                slot_mapping, kvd, k_scale, v_scale, None, scores)
+        return
     _decode(out, query, key_cache, value_cache, num_kv_heads, scale, seq_lens, max_seq_len, slot_mapping, kvd,
             k_scale, v_scale, None, num_splits, maps)
 
@@ -210,11 +262,12 @@ def paged_attention_v1(out, query, key_cache, value_cache, num_kv_heads, scale, 
 def fwd_kvcache(q, k_table_ptr, v_table_ptr, max_seq_len, num_kv_heads, batch, slot_mapping, k_new, v_new,
                 seq_lens, rotary_cos, rotary_sin, cache_batch_idx, block_table, alibi_slopes, out, softmax_scale,
                 causal, window_left, window_right, rotary_interleaved, num_splits, kv_cache_dtype="auto",
-                k_scale=None, v_scale=None):
+                k_scale=None, v_scale=None, scores=None):
     """The 22-positional-argument call the reference's backend makes into its
     flash-attention fork (xformers.py:407-430): q ``[B, 1, H, D]``, pointer-table
     addresses, ``slot_mapping`` slot ids, ``seq_lens`` int32.  Returns ``(out, lse)``
-    with out ``[B, 1, H, D]`` and lse ``[B, H, 1]`` float32.  The arguments the
+    with out ``[B, 1, H, D]`` and lse ``[B, H, 1]`` float32.  ``scores`` accumulates the weights as in
+    :func:`paged_attention_v1` (single-token form).  The arguments the
     reference always passes as None / -1 must be None / -1 here."""
     _require_cuda(q, slot_mapping, seq_lens)
     for name, v in (("k_new", k_new), ("v_new", v_new), ("rotary_cos", rotary_cos), ("rotary_sin", rotary_sin),
@@ -227,6 +280,8 @@ def fwd_kvcache(q, k_table_ptr, v_table_ptr, max_seq_len, num_kv_heads, batch, s
     if q.dim() != 4:
         raise RuntimeError("fwd_kvcache: q must be [B, S, H, D]")
     if q.shape[1] != 1:
+        if scores is not None:
+            raise RuntimeError("fwd_kvcache: scores needs seqlen_q == 1 (prompt_scores serves prompts)")
         # prefix-extend form (xformers.py:362-385): S new tokens per sequence, causal over the range
         if not causal:
             raise RuntimeError("fwd_kvcache: seqlen_q > 1 needs causal=True")
@@ -243,6 +298,10 @@ def fwd_kvcache(q, k_table_ptr, v_table_ptr, max_seq_len, num_kv_heads, batch, s
     q3 = q.view(b, h, d) if q.is_contiguous() else q[:, 0]
     o = out if out is not None else torch.empty(b, 1, h, d, dtype=q.dtype, device=q.device)
     lse = torch.empty(b, h, dtype=torch.float32, device=q.device)
+    if scores is not None:
+        _scored(o.view(b, h, d), q3, None, None, None, k_table_ptr, v_table_ptr, num_kv_heads, softmax_scale, seq_lens,
+                max_seq_len, slot_mapping, _kv_dtype(kv_cache_dtype), k_scale, v_scale, lse, scores)
+        return o, lse.unsqueeze(-1)
     _decode(o.view(b, h, d), q3, k_table_ptr, v_table_ptr, num_kv_heads, softmax_scale, seq_lens, max_seq_len,
             slot_mapping, _kv_dtype(kv_cache_dtype), k_scale, v_scale, lse, 0)
     return o, lse.unsqueeze(-1)
@@ -250,7 +309,7 @@ def fwd_kvcache(q, k_table_ptr, v_table_ptr, max_seq_len, num_kv_heads, batch, s
 
 def decode_step(out, query, key, value, key_cache, value_cache, slot_m, slot_mapping, seq_lens, max_seq_len,
                 num_kv_heads, scale, kv_cache_dtype="auto", k_scale=None, v_scale=None, lse=None, overlap=False,
-                workspace=None, maps=None, clean_scratch=False):
+                workspace=None, maps=None, clean_scratch=False, scores=None):
     """``reshape_and_cache`` (decode form) + ``paged_attention_v1`` in one call; one
     kernel launch for a bf16 cache.  ``key_cache`` / ``value_cache`` are the device
     addresses of the layer's pointer tables (ints), ``slot_m`` the destination byte
@@ -264,13 +323,21 @@ def decode_step(out, query, key, value, key_cache, value_cache, slot_m, slot_map
     ``maps`` (from :func:`decode_maps`, fp8 cache only) selects the tcgen05 kernel where
     the head counts allow; other shapes run as without it.  ``clean_scratch=True``
     (VT_STEP_CLEAN_SCRATCH): ``workspace`` is private, was zero-filled once and is used by
-    nothing but these calls, so the call need not clear its counters first."""
+    nothing but these calls, so the call need not clear its counters first.  ``scores``
+    accumulates the weights as in :func:`paged_attention_v1`; the overlap forms do not apply then,
+    and ``workspace`` comes from ``new_workspace(..., scored=True)``."""
     _require_cuda(out, query, key, value, slot_m, slot_mapping, seq_lens, maps)
     batch, num_heads, head_size = query.shape
     key = key.view(batch, num_kv_heads, head_size)
     value = value.view(batch, num_kv_heads, head_size)
     if overlap and workspace is None:
         raise RuntimeError("decode_step(overlap=True) needs a private zero-filled workspace")
+    if scores is not None:
+        if overlap:
+            raise RuntimeError("decode_step: scores excludes overlap")
+        _scored(out, query, key, value, slot_m, key_cache, value_cache, num_kv_heads, scale, seq_lens, max_seq_len,
+                slot_mapping, _kv_dtype(kv_cache_dtype), k_scale, v_scale, lse, scores, workspace)
+        return
     ws = workspace if workspace is not None else attn_workspace(query.device, batch, num_heads, head_size,
                                                                 max_seq_len)
     flags = (2 if overlap == "early_kv" else (1 if overlap else 0)) | (4 if clean_scratch else 0)
@@ -441,6 +508,81 @@ def prefill_attention(out, query, key_cache, value_cache, num_kv_heads, scale, s
         del holder
 
 
+def prompt_scores(scores, query, key_cache, num_kv_heads, scale, slot_mapping, seq_lens, q_lens, q_start, max_seq_len,
+                  window, kv_cache_dtype="auto", k_scale=None):
+    """Adds the attention weights of a prompt's last queries to ``scores``: what
+    :func:`paged_attention_v1` with ``scores`` adds per decode step, for the last
+    ``min(window, q_lens[i])`` of entry i's new tokens at once.  ``query`` ``[tokens, H, D]`` bf16,
+    ``key_cache`` the address of the K pointer table, ``seq_lens`` / ``q_lens`` / ``q_start`` as in
+    :func:`prefill_attention` (after the rows were appended).  A quantised cache is read back into
+    bf16 scratch first (``k_scale`` needed), at most 1 GiB of it at a time."""
+    _require_cuda(scores, query, slot_mapping, seq_lens, q_lens, q_start, k_scale)
+    if query.dtype != torch.bfloat16 or query.dim() != 3 or query.stride(2) != 1 or query.stride(1) != query.shape[2]:
+        raise RuntimeError("prompt_scores: query must be bfloat16 [tokens, heads, head_size] with contiguous rows")
+    if slot_mapping.dtype != torch.int64 or any(t.dtype != torch.int32 for t in (seq_lens, q_lens, q_start)):
+        raise RuntimeError("prompt_scores: slot_mapping must be int64, seq_lens, q_lens and q_start int32")
+    _check_scores(scores, num_kv_heads, query.device, "prompt_scores")
+    _, num_heads, head_size = query.shape
+    batch, max_seq_len = slot_mapping.numel(), int(max_seq_len)
+    dtype = _kv_dtype(kv_cache_dtype)
+    step, table, range_ids = max(batch, 1), c_void_p(int(key_cache)), None
+    if dtype != VT_KV_BF16:
+        if k_scale is None:
+            raise RuntimeError(f"prompt_scores: an {kv_cache_dtype} cache needs k_scale")
+        row = num_kv_heads * head_size * 2
+        step = max(1, min(step, (1 << 30) // max(1, max_seq_len * row)))
+        rows = torch.empty(step * max_seq_len, num_kv_heads, head_size, dtype=torch.bfloat16, device=query.device)
+        range_ids = torch.arange(step, dtype=torch.int64, device=query.device)
+        bases = range_ids * (max_seq_len * row) + rows.data_ptr()
+        starts = (range_ids * max_seq_len).to(torch.int32)
+        table = _ptr(bases)
+    need = c_size_t()
+    for b in range(0, batch, step):
+        n = min(step, batch - b)
+        slots, lens = slot_mapping[b:b + n], seq_lens[b:b + n]
+        check(lib.vt_prompt_scores_workspace_bytes(n, num_heads, num_kv_heads, head_size, max_seq_len, int(window),
+                                                   byref(need)), "vt_prompt_scores_workspace_bytes")
+        if range_ids is not None:
+            dequantize_ranges(rows, None, key_cache, 0, num_kv_heads, slots, lens, starts[:n], max_seq_len, kv_cache_dtype,
+                              k_scale)
+        ws = _scratch(query.device, need.value + 256)[256:]     # the first word of the scratch is the status word
+        with torch.cuda.device(query.device):
+            check(lib.vt_prompt_scores(_ptr(scores), scores.stride(0), scores.stride(1), scores.shape[2], _ptr(query),
+                                       query.stride(0), table, _ptr(slots), _ptr(range_ids), _ptr(lens),
+                                       _ptr(q_lens[b:b + n]), _ptr(q_start[b:b + n]), n, num_heads, num_kv_heads, head_size,
+                                       max_seq_len, int(window), float(scale), _ptr(ws), ws.numel(), _stream()),
+                  "vt_prompt_scores")
+
+
+def evict_rows(scores, key_cache, value_cache, num_kv_heads, slot_mapping, seq_lens, max_seq_len, budget, sink=0, recent=0,
+               kv_cache_dtype="auto", scores_out=None, head_size=128):
+    """Cuts every sequence longer than ``budget`` rows to ``budget``: per kv head the first ``sink``
+    rows, the last ``recent`` and the heaviest of the others by ``scores`` stay (equal weights: the
+    lower row) and move to the front of their range in their old order; the scores move along
+    (``scores_out``, default in place) and the ones behind become 0.  Returns the old row numbers
+    int32 ``[B, kv_heads, budget]``, -1 behind the rows of a shorter sequence.  The slots of a call
+    must be distinct.  Afterwards the sequences have ``min(seq_lens, budget)`` rows; telling the
+    allocator is the caller's part (``VTensorCacheEngine.evict`` does both)."""
+    _require_cuda(scores, scores_out, slot_mapping, seq_lens)
+    if slot_mapping.dtype != torch.int64 or seq_lens.dtype != torch.int32:
+        raise RuntimeError("evict_rows: slot_mapping must be int64, seq_lens int32")
+    _check_scores(scores, num_kv_heads, slot_mapping.device, "evict_rows")
+    out = scores if scores_out is None else scores_out
+    if out.shape != scores.shape or out.stride() != scores.stride() or out.dtype != scores.dtype or out.device != scores.device:
+        raise RuntimeError("evict_rows: scores_out must be laid out as scores")
+    batch, dtype = slot_mapping.numel(), _kv_dtype(kv_cache_dtype)
+    need = c_size_t()
+    check(lib.vt_evict_workspace_bytes(batch, num_kv_heads, int(budget), dtype, byref(need)), "vt_evict_workspace_bytes")
+    kept = torch.empty(batch, num_kv_heads, int(budget), dtype=torch.int32, device=scores.device)
+    ws = _scratch(scores.device, need.value)
+    with torch.cuda.device(scores.device):
+        check(lib.vt_evict_rows(_ptr(scores), _ptr(out), scores.stride(0), scores.stride(1), scores.shape[2],
+                                c_void_p(int(key_cache)), c_void_p(int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens),
+                                batch, num_kv_heads, head_size, int(max_seq_len), int(budget), int(sink), int(recent), dtype,
+                                _ptr(kept), _ptr(ws), ws.numel(), _stream()), "vt_evict_rows")
+    return kept
+
+
 def attn_plan(batch, num_heads, num_kv_heads, max_seq_len, kv_cache_dtype="auto", num_splits=0):
     """(tokens per partition, partitions per sequence, kernel variant) the library
     picks for this problem size."""
@@ -471,10 +613,5 @@ def workspace_status(workspace):
 def attn_status(device=None):
     """VT_OK (0) unless an attention kernel's bounded wait ran out since the
     workspace was created.  Synchronises the current stream."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else device
-    ws = _workspaces.get(dev.index if dev.index is not None else torch.cuda.current_device())
-    if ws is None:
-        return 0
-    code = ctypes.c_int()
-    check(lib.vt_decode_attn_status(_ptr(ws), _stream(), byref(code)), "vt_decode_attn_status")
-    return code.value
+    dev = torch.cuda.current_device() if device is None else _device_index(device)
+    return max((workspace_status(ws) for (index, _), ws in list(_workspaces.items()) if index == dev), default=0)

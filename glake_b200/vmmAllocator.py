@@ -190,6 +190,15 @@ class KVcacheSegment:
         keep = self.expand_size if self.actual_size >= self.expand_size else 0
         check(lib.vt_seg_release(self._h, int(keep)), "vt_seg_release")
 
+    def trim(self, used_size, keep_size=0):
+        """Shortens the sequence to its first ``used_size`` bytes per range and unmaps whole chunks
+        behind ``max(used_size, keep_size)`` and the pre-cached prefix.  No kernel that reads the
+        rows behind may be in flight.  (No counterpart in the reference, whose sequences only grow.)"""
+        self.wait()
+        keep = max(int(used_size), int(keep_size), self.expand_size if self.actual_size >= self.expand_size else 0)
+        check(lib.vt_seg_release(self._h, keep), "vt_seg_release")
+        self.set_used_size(int(used_size))
+
     def preempt_seq(self, seq_id):
         """Unmap everything (vmm_allocator.cpp:348-381)."""
         _slot_registry.pop(int(seq_id), None)

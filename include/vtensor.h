@@ -350,6 +350,66 @@ int vt_decode_step_tma(void *out, int64_t out_stride, const void *q, int64_t q_s
                        int kv_dtype, const float *k_scale, const float *v_scale, float *lse, void *workspace,
                        size_t workspace_bytes, unsigned flags, const void *maps, void *stream);
 
+/* vt_decode_step (or, with key and value NULL, vt_decode_attn) that also accumulates what every
+ * cached row received: for every entry i, kv head j and row t < seq_lens[i]
+ *   scores[slot_ids[i] * score_slot_stride + j * score_head_stride + t] +=
+ *       sum over the q heads of kv head j of the softmax weight of row t
+ * scores is device float, strides in elements, rows contiguous, score_rows of them per (slot,
+ * kv head); max_seq_len must bound every seq_lens[i] (a longer context is cut there) and may not
+ * exceed score_rows.  Rows at and behind seq_lens[i] are left as they are.  Nothing is read or
+ * written for slots that no entry names; a slot named by two entries receives both.  Two
+ * launches: the attention kernels write logits and softmax statistics into the workspace
+ * (vt_decode_scored_workspace_bytes, 256-byte aligned, content irrelevant), a second kernel adds
+ * the weights.  All cache types and head shapes of vt_decode_step.  No counterpart in the reference. */
+int vt_decode_scored_workspace_bytes(int batch, int h, int d, int max_seq_len, size_t *bytes);
+int vt_decode_step_scored(void *out, int64_t out_stride, const void *q, int64_t q_stride, const void *key,
+                          const void *value, int64_t key_stride, int64_t value_stride, const int64_t *byte_off,
+                          const uint64_t *k_table, const uint64_t *v_table, const int64_t *slot_ids,
+                          const int32_t *seq_lens, int batch, int h, int kvh, int d, int max_seq_len, float scale,
+                          int kv_dtype, const float *k_scale, const float *v_scale, float *lse, float *scores,
+                          int64_t score_slot_stride, int64_t score_head_stride, int score_rows, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/* Adds the attention weights of a prompt's last queries to scores (laid out as in
+ * vt_decode_step_scored): with w = min(window, q_lens[i], seq_lens[i]), the last w of entry i's new
+ * tokens, query j of them seeing rows 0 .. seq_lens[i] - w + j, each add their softmax weights,
+ * summed over the q heads of a kv head.
+ *   q           bf16 [tokens, h, d], row stride in elements (even), 4-byte aligned; q_lens / q_start as
+ *               in vt_prefill_attn
+ *   k_table     bf16 ranges; range_ids (device int64 [batch]) index it, NULL = slot_ids.  A quantised
+ *               cache is read back first (vt_kv_dequant) and named through range_ids
+ *   workspace   vt_prompt_scores_workspace_bytes, 256-byte aligned, content irrelevant
+ * max_seq_len bounds seq_lens (a longer context is cut there) and is at most score_rows;
+ * window * h / kvh <= 16384.  No counterpart in the reference. */
+int vt_prompt_scores_workspace_bytes(int batch, int h, int kvh, int d, int max_seq_len, int window, size_t *bytes);
+int vt_prompt_scores(float *scores, int64_t score_slot_stride, int64_t score_head_stride, int score_rows, const void *q,
+                     int64_t q_stride, const uint64_t *k_table, const int64_t *slot_ids, const int64_t *range_ids,
+                     const int32_t *seq_lens, const int32_t *q_lens, const int32_t *q_start, int batch, int h, int kvh,
+                     int d, int max_seq_len, int window, float scale, void *workspace, size_t workspace_bytes,
+                     void *stream);
+
+/* Evicts rows from the ranges of one layer.  Every entry i with n = seq_lens[i] > budget keeps, per
+ * kv head, its first `sink` rows, its last `recent` rows and, of the others, the
+ * budget - sink - recent with the largest scores (equal scores: the lower row; NaN counts as
+ * -inf).  The kept rows of K and V move to rows 0 .. budget - 1 of their range in their old order;
+ * rows behind are not touched (the caller shortens the sequence to min(n, budget) rows and may
+ * release the memory behind them).
+ *   kept        device int32 [batch, kvh, budget]: the old row numbers, ascending; an entry with
+ *               n <= budget gets 0 .. n - 1 and then -1, and none of its rows moves
+ *   scores_out  same layout as scores, or scores itself (no other overlap): rows 0 .. min(n, budget) - 1
+ *               get the kept rows' scores, rows up to n become 0, rows behind n are left as they are
+ *   workspace   vt_evict_workspace_bytes, 256-byte aligned; its first word reads as vt_decode_attn_status
+ *               says (a bounded wait that ran out leaves the ranges undefined)
+ * slot_ids must be distinct: two entries that name one slot would move its rows at the same time.
+ * All cache types; in place, no second copy of the rows.  sink + recent <= budget; max_seq_len
+ * bounds seq_lens (a longer context is cut there) and is at most score_rows.  Two launches.  No
+ * counterpart in the reference. */
+int vt_evict_workspace_bytes(int batch, int kvh, int budget, int kv_dtype, size_t *bytes);
+int vt_evict_rows(const float *scores, float *scores_out, int64_t score_slot_stride, int64_t score_head_stride,
+                  int score_rows, const uint64_t *k_table, const uint64_t *v_table, const int64_t *slot_ids,
+                  const int32_t *seq_lens, int batch, int kvh, int d, int max_seq_len, int budget, int sink, int recent,
+                  int kv_dtype, int32_t *kept, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Causal attention of the NEW tokens of each sequence over its whole range
  * (prefix + new tokens; the new rows must have been appended with vt_append):
  * query row j of entry i sits at position seq_lens[i] - q_lens[i] + j and attends

@@ -60,6 +60,8 @@ def unpack4(rows, kvh, scale):
 def encode(x, kv, scale):
     """bf16 rows [n, kvh, 128] on the CPU -> cache bytes [n, row bytes]."""
     n, kvh, _ = x.shape
+    if n == 0:
+        return torch.zeros(0, row_bytes(kvh, kv), dtype=torch.uint8)
     if kv == "int4":
         return pack4(x, scale)
     if kv == "fp8_e4m3":
@@ -69,6 +71,8 @@ def encode(x, kv, scale):
 
 def decode(rows, kv, kvh, scale):
     """Cache bytes [n, row bytes] on the CPU -> float64 [n, kvh, 128]."""
+    if rows.shape[0] == 0:
+        return torch.zeros(0, kvh, D, dtype=torch.float64)
     if kv == "int4":
         return unpack4(rows, kvh, scale)
     if kv == "fp8_e4m3":

@@ -35,7 +35,7 @@ namespace vt {
 namespace {
 
 constexpr int kCWarps = 8;                 // consumer warps = heads of a unit x token sub-rows of a tile
-constexpr int kThreads4 = (kCWarps + 1) * 32;
+constexpr int kThreads4 = kCWarps * 32;
 constexpr int kRingBudget = 106000;        // two CTAs per SM with their tables
 constexpr int kBaseCacheMaxBatch4 = 256;
 constexpr float kPScaleLog2 = 6.f;         // P is carried times 2^6
@@ -52,6 +52,13 @@ struct Cfg4 {
   static_assert(kStages >= 3, "ring too shallow");
 };
 
+// 2^x to about 2 ulp; 0 for -inf.  (Below 2^-126 it flushes to 0, far under what a probability contributes.)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // fragment row -> token of the warp's 16 (see the header: conflict-free at the pitch of U heads)
 template <int U>
 __device__ __forceinline__ int token_of_row(int row) {
@@ -61,10 +68,18 @@ __device__ __forceinline__ int token_of_row(int row) {
   return static_cast<int>((0xA684E2C0u >> (4 * i)) & 15u) + (row >> 3);   // pitches 68, 36, 20 words = 4 mod 16 (odd x 4)
 }
 
+// D = A B, accumulator starting at zero
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 template <int NB>
 struct WarpAttn4 {
   uint32_t qb[NB][4][2][2];   // [group][step][k half]
-  float qoff[NB][4][2];       // start value of the logit accumulators: -8 sum q, per column
+  float qoff[NB][4][2];       // -8 sum q over the group, per column
   float qmul[NB][2];          // partial logits -> log2 domain
   float o[NB][8][4];
   float corr[NB][4];          // row G: 8 sum p s_v[G]
@@ -112,7 +127,7 @@ struct WarpAttn4 {
         sum[G] += __shfl_xor_sync(0xffffffffu, sum[G], 1);
         sum[G] += __shfl_xor_sync(0xffffffffu, sum[G], 2);
       }
-      const float mul = sl2 * (4294967296.f / f);   // 2^24 of the nibbles, 2^8 of the scales, 1 / f of Q
+      const float mul = sl2 * (16777216.f / f);   // 2^24 of the nibbles, 1 / f of Q
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int src = (2 * c4 + e) * 4;
@@ -128,127 +143,79 @@ struct WarpAttn4 {
     }
   }
 
-  // 16 tokens of the tile: kt / vt = the head's K / V bytes of token 0 of the 16, sc = offset of the scale words from
-  // there, n_tok = how many of the 16 (in token order) are inside the context.
-  template <int U, bool LOG>
-  __device__ __forceinline__ void step(const unsigned char *kt, const unsigned char *vt, int sc, int n_tok, int lane,
-                                       float *lg, int g) {
+  // Partial logits of 16 tokens per group of dims, joined with the group scales: s[nb][token ta: heads 2 c4, + 1; tb: ..].
+  template <int U>
+  __device__ __forceinline__ void logits(float (&s)[NB][4], const unsigned char *kt, int sc, int ta, int tb, int c4) const {
     constexpr int UB = Cfg4<U>::UB;
-    const int r4 = lane >> 2, c4 = lane & 3;
-    const int ta = token_of_row<U>(r4), tb = token_of_row<U>(r4 + 8);
-    // ---- partial logits per group ----
-    float s[NB][4];
-    {
-      float acc[NB][4][4];
+    float acc[NB][4][4];
+    const uint4 ka = *reinterpret_cast<const uint4 *>(kt + ta * UB + 16 * c4);
+    const uint4 kb = *reinterpret_cast<const uint4 *>(kt + tb * UB + 16 * c4);
+    const uint32_t wsa = *reinterpret_cast<const uint32_t *>(kt + ta * UB + sc);
+    const uint32_t wsb = *reinterpret_cast<const uint32_t *>(kt + tb * UB + sc);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+    for (int G = 0; G < 4; ++G) {
+      const uint32_t sel = (G & 1) ? 0x7632u : 0x5410u;
+      uint32_t xa = G < 2 ? prmt(ka.x, ka.z, sel) : prmt(ka.y, ka.w, sel);
+      uint32_t xb = G < 2 ? prmt(kb.x, kb.z, sel) : prmt(kb.y, kb.w, sel);
 #pragma unroll
-        for (int G = 0; G < 4; ++G) {
-          acc[nb][G][0] = acc[nb][G][2] = qoff[nb][G][0];
-          acc[nb][G][1] = acc[nb][G][3] = qoff[nb][G][1];
+      for (int a = 0; a < 2; ++a) {
+        const uint32_t f[4] = {xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u};
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          if (a == 0) mma_f16_zero(acc[nb][G], f, qb[nb][G][0][0], qb[nb][G][0][1]);
+          else mma_f16(acc[nb][G], f, qb[nb][G][1][0], qb[nb][G][1][1]);
         }
-      const uint4 ka = *reinterpret_cast<const uint4 *>(kt + ta * UB + 16 * c4);
-      const uint4 kb = *reinterpret_cast<const uint4 *>(kt + tb * UB + 16 * c4);
-      const uint32_t wsa = *reinterpret_cast<const uint32_t *>(kt + ta * UB + sc);
-      const uint32_t wsb = *reinterpret_cast<const uint32_t *>(kt + tb * UB + sc);
-#pragma unroll
-      for (int G = 0; G < 4; ++G) {
-        const uint32_t sel = (G & 1) ? 0x7632u : 0x5410u;
-        uint32_t xa = G < 2 ? prmt(ka.x, ka.z, sel) : prmt(ka.y, ka.w, sel);
-        uint32_t xb = G < 2 ? prmt(kb.x, kb.z, sel) : prmt(kb.y, kb.w, sel);
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const uint32_t f[4] = {xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u};
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma_f16(acc[nb][G], f, qb[nb][G][a][0], qb[nb][G][a][1]);
-          xa >>= 8;
-          xb >>= 8;
-        }
-      }
-      // e4m3 (sign 0) << 7 is the f16 of the value times 2^-8
-      const uint32_t a01 = prmt(wsa, 0u, 0x4140u) << 7, a23 = prmt(wsa, 0u, 0x4342u) << 7;
-      const uint32_t b01 = prmt(wsb, 0u, 0x4140u) << 7, b23 = prmt(wsb, 0u, 0x4342u) << 7;
-      const float ga[4] = {f16_lo(a01), f16_hi(a01), f16_lo(a23), f16_hi(a23)};
-      const float gb[4] = {f16_lo(b01), f16_hi(b01), f16_lo(b23), f16_hi(b23)};
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nb][e] = 0.f;
-#pragma unroll
-        for (int G = 0; G < 4; ++G) {
-          s[nb][0] = fmaf(ga[G], acc[nb][G][0], s[nb][0]);
-          s[nb][1] = fmaf(ga[G], acc[nb][G][1], s[nb][1]);
-          s[nb][2] = fmaf(gb[G], acc[nb][G][2], s[nb][2]);
-          s[nb][3] = fmaf(gb[G], acc[nb][G][3], s[nb][3]);
-        }
+        xa >>= 8;
+        xb >>= 8;
       }
     }
-    // ---- online softmax (rows = tokens ta, tb; columns = heads 2 c4, 2 c4 + 1) ----
-    const bool va = ta < n_tok, vb = tb < n_tok;
-    uint32_t pb[NB][2];
-    float fac[NB][2];
-    bool any_up = false;
+    const uint32_t a01 = e4m3x2_to_f16x2(wsa), a23 = e4m3x2_to_f16x2(wsa >> 16);
+    const uint32_t b01 = e4m3x2_to_f16x2(wsb), b23 = e4m3x2_to_f16x2(wsb >> 16);
+    const float ga[4] = {f16_lo(a01), f16_hi(a01), f16_lo(a23), f16_hi(a23)};
+    const float gb[4] = {f16_lo(b01), f16_hi(b01), f16_lo(b23), f16_hi(b23)};
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const float s00 = va ? s[nb][0] * qmul[nb][0] : -INFINITY, s01 = va ? s[nb][1] * qmul[nb][1] : -INFINITY;
-      const float s10 = vb ? s[nb][2] * qmul[nb][0] : -INFINITY, s11 = vb ? s[nb][3] * qmul[nb][1] : -INFINITY;
-      if constexpr (LOG) {
-        const int head = nb * 8 + 2 * c4;
-        if (head + 1 < g) {   // head is even, and so is g here: 8-byte aligned
-          if (va) *reinterpret_cast<float2 *>(lg + ta * g + head) = make_float2(s00, s01);
-          if (vb) *reinterpret_cast<float2 *>(lg + tb * g + head) = make_float2(s10, s11);
-        } else if (head < g) {
-          if (va) lg[ta * g + head] = s00;
-          if (vb) lg[tb * g + head] = s10;
-        }
-      }
-      float mx0 = fmaxf(s00, s10), mx1 = fmaxf(s01, s11);
+      // the "- 8" of a group is added to its sum here, on the FMA pipe: as the start value of the accumulators it
+      // costs a move per register on the ALU pipe, which is the busy one
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
-      }
-      // the running "maximum" sits 6 below the true one, which carries P times 2^6 through sums, states and merges
-      const float mn0 = fmaxf(mrun[nb][0], mx0 - kPScaleLog2), mn1 = fmaxf(mrun[nb][1], mx1 - kPScaleLog2);
-      fac[nb][0] = exp2f(mrun[nb][0] - mn0);   // token 0 of the 16 is valid, so mn is finite
-      fac[nb][1] = exp2f(mrun[nb][1] - mn1);
-      any_up |= (mn0 > mrun[nb][0]) | (mn1 > mrun[nb][1]);
-      mrun[nb][0] = mn0;
-      mrun[nb][1] = mn1;
-      const float p00 = exp2f(s00 - mn0), p01 = exp2f(s01 - mn1), p10 = exp2f(s10 - mn0), p11 = exp2f(s11 - mn1);
-      lrun[nb][0] = lrun[nb][0] * fac[nb][0] + p00 + p10;
-      lrun[nb][1] = lrun[nb][1] * fac[nb][1] + p01 + p11;
-      pb[nb][0] = movmatrix_trans(pack_f16(p00, p01));
-      pb[nb][1] = movmatrix_trans(pack_f16(p10, p11));
-    }
-    if (__any_sync(0xffffffffu, any_up)) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int mb = 0; mb < 8; ++mb) {
-          o[nb][mb][0] *= fac[nb][0]; o[nb][mb][1] *= fac[nb][1];
-          o[nb][mb][2] *= fac[nb][0]; o[nb][mb][3] *= fac[nb][1];
-        }
-        corr[nb][0] *= fac[nb][0]; corr[nb][1] *= fac[nb][1];
+      for (int G = 0; G < 4; ++G) {
+        const float x0 = acc[nb][G][0] + qoff[nb][G][0], x1 = acc[nb][G][1] + qoff[nb][G][1];
+        const float x2 = acc[nb][G][2] + qoff[nb][G][0], x3 = acc[nb][G][3] + qoff[nb][G][1];
+        s[nb][0] = G ? fmaf(ga[G], x0, s[nb][0]) : ga[G] * x0;
+        s[nb][1] = G ? fmaf(ga[G], x1, s[nb][1]) : ga[G] * x1;
+        s[nb][2] = G ? fmaf(gb[G], x2, s[nb][2]) : gb[G] * x2;
+        s[nb][3] = G ? fmaf(gb[G], x3, s[nb][3]) : gb[G] * x3;
       }
     }
-    // ---- O^T += V^T . (s_v P)^T ----
+  }
+
+  // O^T += V^T . (s_v P)^T over 16 tokens; pb = P^T as a B operand.
+  template <int U>
+  __device__ __forceinline__ void values(const uint32_t (&pb)[NB][2], const unsigned char *vt, int sc, int n_tok, int r4, int c4) {
+    constexpr int UB = Cfg4<U>::UB;
     const int t0 = token_of_row<U>(2 * c4), t1 = token_of_row<U>(2 * c4 + 1);
     const int t2 = token_of_row<U>(2 * c4 + 8), t3 = token_of_row<U>(2 * c4 + 9);
     const uint2 v0 = *reinterpret_cast<const uint2 *>(vt + t0 * UB + 8 * r4);
     const uint2 v1 = *reinterpret_cast<const uint2 *>(vt + t1 * UB + 8 * r4);
     const uint2 v2 = *reinterpret_cast<const uint2 *>(vt + t2 * UB + 8 * r4);
     const uint2 v3 = *reinterpret_cast<const uint2 *>(vt + t3 * UB + 8 * r4);
-    // sign bits cleared: what lies past the context is stale, and shifted it must stay finite (its P is 0)
-    const uint32_t w0 = *reinterpret_cast<const uint32_t *>(vt + t0 * UB + sc) & 0x7f7f7f7fu;
-    const uint32_t w1 = *reinterpret_cast<const uint32_t *>(vt + t1 * UB + sc) & 0x7f7f7f7fu;
-    const uint32_t w2 = *reinterpret_cast<const uint32_t *>(vt + t2 * UB + sc) & 0x7f7f7f7fu;
-    const uint32_t w3 = *reinterpret_cast<const uint32_t *>(vt + t3 * UB + sc) & 0x7f7f7f7fu;
+    uint32_t w0 = *reinterpret_cast<const uint32_t *>(vt + t0 * UB + sc);
+    uint32_t w1 = *reinterpret_cast<const uint32_t *>(vt + t1 * UB + sc);
+    uint32_t w2 = *reinterpret_cast<const uint32_t *>(vt + t2 * UB + sc);
+    uint32_t w3 = *reinterpret_cast<const uint32_t *>(vt + t3 * UB + sc);
+    if (n_tok < 16) {   // what lies past the context is stale and may be NaN as a scale; its P is 0
+      w0 = t0 < n_tok ? w0 : 0u;
+      w1 = t1 < n_tok ? w1 : 0u;
+      w2 = t2 < n_tok ? w2 : 0u;
+      w3 = t3 < n_tok ? w3 : 0u;
+    }
+    // per pair of tokens the scale bytes of groups (0, 1) and (2, 3), interleaved
+    const uint32_t y01[2] = {prmt(w0, w1, 0x5140u), prmt(w0, w1, 0x7362u)};
+    const uint32_t y23[2] = {prmt(w2, w3, 0x5140u), prmt(w2, w3, 0x7362u)};
 #pragma unroll
     for (int G = 0; G < 4; ++G) {
-      // bytes (a.G, 0, b.G, 0): selector bit 3 replicates the (clear) sign bit
-      const uint32_t sel = G | (8u | G) << 4 | (4u + G) << 8 | (12u + G) << 12;
-      const uint32_t s01 = prmt(w0, w1, sel) << 7, s23 = prmt(w2, w3, sel) << 7;
+      const uint32_t s01 = e4m3x2_to_f16x2((G & 1) ? y01[G >> 1] >> 16 : y01[G >> 1]);
+      const uint32_t s23 = e4m3x2_to_f16x2((G & 1) ? y23[G >> 1] >> 16 : y23[G >> 1]);
       uint32_t b0[NB], b1[NB];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
@@ -275,11 +242,96 @@ struct WarpAttn4 {
     }
   }
 
+  // One tile of this warp: SUBS x 16 tokens, `stride` tokens apart.  kt / vt = the head's K / V bytes of the first
+  // token, sc = offset of the scale words from there, n_tok > 0 = tokens from that one to the end of the context.
+  template <int U, bool LOG>
+  __device__ __forceinline__ void tile(const unsigned char *kt, const unsigned char *vt, int sc, int n_tok, int lane, float *lg,
+                                       int g) {
+    constexpr int SUBS = Cfg4<U>::SUBS, STEP = 16 * Cfg4<U>::R, UB = Cfg4<U>::UB;
+    const int r4 = lane >> 2, c4 = lane & 3;
+    const int ta = token_of_row<U>(r4), tb = token_of_row<U>(r4 + 8);
+    float s[SUBS][NB][4];
+#pragma unroll
+    for (int i = 0; i < SUBS; ++i) logits<U>(s[i], kt + i * STEP * UB, sc, ta, tb, c4);
+    // ---- online softmax (rows = tokens ta, tb; columns = heads 2 c4, 2 c4 + 1) ----
+    uint32_t pb[SUBS][NB][2];
+    float fac[NB][2];
+    bool any_up = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < SUBS; ++i) {
+        float(&x)[4] = s[i][nb];
+        x[0] *= qmul[nb][0];
+        x[1] *= qmul[nb][1];
+        x[2] *= qmul[nb][0];
+        x[3] *= qmul[nb][1];
+        const bool va = ta + i * STEP < n_tok, vb = tb + i * STEP < n_tok;
+        if (n_tok < (SUBS - 1) * STEP + 16) {   // the context ends in this tile
+          x[0] = va ? x[0] : -INFINITY;
+          x[1] = va ? x[1] : -INFINITY;
+          x[2] = vb ? x[2] : -INFINITY;
+          x[3] = vb ? x[3] : -INFINITY;
+        }
+        if constexpr (LOG) {
+          const int head = nb * 8 + 2 * c4;
+          float *pa = lg + (ta + i * STEP) * g + head, *pt = lg + (tb + i * STEP) * g + head;
+          if (head + 1 < g) {   // head is even, and so is g here: 8-byte aligned
+            if (va) *reinterpret_cast<float2 *>(pa) = make_float2(x[0], x[1]);
+            if (vb) *reinterpret_cast<float2 *>(pt) = make_float2(x[2], x[3]);
+          } else if (head < g) {
+            if (va) *pa = x[0];
+            if (vb) *pt = x[2];
+          }
+        }
+        mx0 = fmaxf(mx0, fmaxf(x[0], x[2]));
+        mx1 = fmaxf(mx1, fmaxf(x[1], x[3]));
+      }
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+      }
+      // the running "maximum" sits 6 below the true one, which carries P times 2^6 through sums, states and merges
+      const float mn0 = fmaxf(mrun[nb][0], mx0 - kPScaleLog2), mn1 = fmaxf(mrun[nb][1], mx1 - kPScaleLog2);
+      fac[nb][0] = ex2(mrun[nb][0] - mn0);   // the first token is valid, so mn is finite
+      fac[nb][1] = ex2(mrun[nb][1] - mn1);
+      any_up |= (mn0 > mrun[nb][0]) | (mn1 > mrun[nb][1]);
+      mrun[nb][0] = mn0;
+      mrun[nb][1] = mn1;
+      lrun[nb][0] *= fac[nb][0];
+      lrun[nb][1] *= fac[nb][1];
+#pragma unroll
+      for (int i = 0; i < SUBS; ++i) {
+        const float(&x)[4] = s[i][nb];
+        const float p00 = ex2(x[0] - mn0), p01 = ex2(x[1] - mn1), p10 = ex2(x[2] - mn0), p11 = ex2(x[3] - mn1);
+        lrun[nb][0] += p00 + p10;
+        lrun[nb][1] += p01 + p11;
+        pb[i][nb][0] = movmatrix_trans(pack_f16(p00, p01));
+        pb[i][nb][1] = movmatrix_trans(pack_f16(p10, p11));
+      }
+    }
+    if (__any_sync(0xffffffffu, any_up)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int mb = 0; mb < 8; ++mb) {
+          o[nb][mb][0] *= fac[nb][0]; o[nb][mb][1] *= fac[nb][1];
+          o[nb][mb][2] *= fac[nb][0]; o[nb][mb][3] *= fac[nb][1];
+        }
+        corr[nb][0] *= fac[nb][0]; corr[nb][1] *= fac[nb][1];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < SUBS; ++i) values<U>(pb[i], vt + i * STEP * UB, sc, n_tok - i * STEP, r4, c4);
+  }
+
   // Row sums over the lanes, the "- 8" correction and the powers of two: afterwards o and lrun are what the
   // other engines publish (the head scale of V is applied by the merge).
   __device__ __forceinline__ void finish(int lane) {
     const int c4 = lane & 3;
-    constexpr float kLo = 4294967296.f;   // 2^24 of the nibbles, 2^8 of the scales; row r4 + 8 holds upper nibbles: a sixteenth
+    constexpr float kLo = 16777216.f;   // 2^24 of the nibbles; row r4 + 8 holds upper nibbles: a sixteenth
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -326,11 +378,18 @@ struct WarpAttn4 {
   }
 };
 
-// ring | barriers | flags | prefix[batch + 1] | lens[batch] | (pad to 8) | kbase[batch] | vbase[batch]
+// Where a warp's copies stand: the tile to fetch next.  In shared memory: it is needed once per tile, registers always.
+struct Cursor {
+  const char *k, *v;         // the unit's rows of the piece's sequence
+  long long tau;             // position of the piece after this one
+  int tile, tile_end, seq_len, pad;
+};
+
+// ring | barriers | cursors | flags | prefix[batch + 1] | lens[batch] | (pad to 8) | kbase[batch] | vbase[batch]
 __host__ __device__ constexpr int meta_ints4(int batch) { return ((2 * batch + 1 + 4) + 1) / 2 * 2; }
 template <int U>
 constexpr int smem_bytes4(int batch) {
-  return Cfg4<U>::kStages * (Cfg4<U>::kStage + 16) + meta_ints4(batch) * 4 + (batch <= kBaseCacheMaxBatch4 ? batch * 16 : 0);
+  return Cfg4<U>::kStages * (Cfg4<U>::kStage + 16) + kCWarps * static_cast<int>(sizeof(Cursor)) + meta_ints4(batch) * 4 + (batch <= kBaseCacheMaxBatch4 ? batch * 16 : 0);
 }
 
 template <int U, int NB, bool LOG>
@@ -339,7 +398,9 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(A
   constexpr int R = C::R, UB = C::UB, TOK = C::TOK, HEADS = NB * 8;
   extern __shared__ __align__(128) unsigned char smem[];
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kStages * C::kStage);
-  int *flags = reinterpret_cast<int *>(bars + 2 * C::kStages);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Cursor &cur = reinterpret_cast<Cursor *>(bars + 2 * C::kStages)[warp];
+  int *flags = reinterpret_cast<int *>(reinterpret_cast<Cursor *>(bars + 2 * C::kStages) + kCWarps);
   int *prefix = flags + 4;
   int *lens = prefix + p.batch + 1;
   const bool cache_bases = p.batch <= kBaseCacheMaxBatch4;
@@ -348,10 +409,9 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(A
   const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + C::kStages), ring0 = smem_u32(smem);
 
   const int g = p.h / p.kvh, slabs = p.kvh / U;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full0 + 8 * s, 1);
+      mbar_init(full0 + 8 * s, kCWarps);
       mbar_init(empty0 + 8 * s, kCWarps);
     }
     mbar_fence_init();
@@ -392,48 +452,68 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(A
   const long long tau1 = active ? total * (blockIdx.x + 1) / n_ctas : 0;
   const int64_t row_bytes = static_cast<int64_t>(slabs) * UB;
 
-  if (warp == kCWarps) {
-    // ---------------- producer warp ----------------
-    // A single-unit cache is contiguous over tokens: one copy of K and one of V per tile.  Otherwise a row of the
-    // unit (80 to 544 bytes) is one copy.
-    const uint64_t policy = l2_policy_evict_first();
-    int it = 0;
-    for (long long tau = tau0; tau < tau1;) {
-      const Piece pc = locate(prefix, p.batch, slabs, tau, tau1);
-      const int seq_len = lens[pc.b];
-      const char *kb, *vb;
-      if (cache_bases) {
-        kb = reinterpret_cast<const char *>(kbase_s[pc.b]);
-        vb = reinterpret_cast<const char *>(vbase_s[pc.b]);
-      } else {
-        const int64_t slot = p.slot_ids[pc.b];
-        kb = reinterpret_cast<const char *>(p.k_table[slot]);
-        vb = reinterpret_cast<const char *>(p.v_table[slot]);
+  // ---------------- copies ----------------
+  // Every warp fetches an eighth of the rows of the CTA's next tile into its ring stage, `n` tiles into the share, once
+  // all warps are done with what the stage held; false when a bounded wait ran out.  A single-unit cache is contiguous
+  // over tokens: one copy of K and one of V.  Otherwise a row of the unit (80 to 544 bytes) is one copy, a lane each.
+  const uint64_t policy = l2_policy_evict_first();
+  const auto fetch = [&](int n) -> bool {
+    if (cur.tile >= cur.tile_end) {
+      long long tau = cur.tau;
+      Piece pc{};
+      while (tau < tau1) {
+        pc = locate(prefix, p.batch, slabs, tau, tau1);
+        tau += pc.advance;
+        if (pc.tile_end > pc.tile_begin) break;
       }
-      for (int tile = pc.tile_begin; tile < pc.tile_end; ++tile, ++it) {
-        const int s = it % C::kStages;
-        if (it >= C::kStages && !mbar_wait(empty0 + 8 * s, ((it / C::kStages) - 1) & 1)) {
-          if (lane == 0) atomicExch(p.status, kKernelErrMagic);
-          return;
-        }
-        const int t0 = tile * TOK, nt = min(TOK, seq_len - t0);
-        if (lane == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2u * nt * UB);
-        __syncwarp();
-        const uint32_t dst = ring0 + s * C::kStage;
-        const int64_t src = t0 * row_bytes + pc.slab * UB;
-        if (slabs == 1) {
-          if (lane < 2) bulk_g2s_hint(dst + lane * C::kTile, (lane ? vb : kb) + src, nt * UB, full0 + 8 * s, policy);
-        } else {
-          for (int i = lane; i < 2 * nt; i += 32) {
-            const int v = i >= nt, t = v ? i - nt : i;
-            bulk_g2s_hint(dst + v * C::kTile + t * UB, (v ? vb : kb) + src + t * row_bytes, UB, full0 + 8 * s, policy);
-          }
+      __syncwarp();
+      if (lane == 0) {
+        cur.tau = tau;
+        cur.tile = pc.tile_begin;
+        cur.tile_end = pc.tile_end;
+        if (pc.tile_end > pc.tile_begin) {
+          const int64_t slot = p.slot_ids[pc.b];
+          cur.k = reinterpret_cast<const char *>(cache_bases ? kbase_s[pc.b] : p.k_table[slot]) + pc.slab * UB;
+          cur.v = reinterpret_cast<const char *>(cache_bases ? vbase_s[pc.b] : p.v_table[slot]) + pc.slab * UB;
+          cur.seq_len = lens[pc.b];
         }
       }
-      tau += pc.advance;
+      __syncwarp();
+      if (cur.tile >= cur.tile_end) return true;   // the share is fetched
     }
-    return;
+    constexpr int ROWS = TOK / kCWarps;
+    const int tile = cur.tile, s = n % C::kStages;
+    const int t0 = tile * TOK + warp * ROWS, nt = min(max(cur.seq_len - t0, 0), ROWS);
+    const int64_t src = t0 * row_bytes;
+    const char *kb = cur.k + src, *vb = cur.v + src;
+    if (n >= C::kStages && !mbar_wait(empty0 + 8 * s, ((n / C::kStages) - 1) & 1)) {
+      if (lane == 0) atomicExch(p.status, kKernelErrMagic);
+      return false;
+    }
+    const uint32_t dst = ring0 + s * C::kStage + warp * ROWS * UB;
+    __syncwarp();
+    if (lane == 0) {
+      cur.tile = tile + 1;
+      mbar_arrive_expect_tx(full0 + 8 * s, 2u * nt * UB);
+    }
+    __syncwarp();
+    if (slabs == 1) {
+      if (lane < 2 && nt > 0) bulk_g2s_hint(dst + lane * C::kTile, lane ? vb : kb, nt * UB, full0 + 8 * s, policy);
+    } else {
+      const int row = lane & 15;
+      static_assert(ROWS <= 16, "a lane per row of K and of V");
+      if (row < nt)
+        bulk_g2s_hint(dst + (lane >> 4) * C::kTile + row * UB, (lane >> 4 ? vb : kb) + row * row_bytes, UB, full0 + 8 * s, policy);
+    }
+    return true;
+  };
+  bool failed = false;
+  if (lane == 0) {
+    cur.tau = tau0;
+    cur.tile = cur.tile_end = 0;
   }
+  __syncwarp();
+  for (int n = 0; n < C::kStages - 1; ++n) failed |= !fetch(n);
 
   // ---------------- consumer warps ----------------
   const int hs = warp % U, rr = warp / U;
@@ -448,7 +528,6 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(A
           for (int i = tid; i < p.h; i += kCWarps * 32) p.lse[b * p.h + i] = -INFINITY;
       }
   }
-  bool failed = false;
   int it = 0;
   bool first_piece = true;
   for (long long tau = tau0; tau < tau1;) {
@@ -468,6 +547,8 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(A
     if constexpr (LOG) lg = p.logits + (static_cast<size_t>(pc.b) * p.kvh + kv_head) * p.logit_rows * g;
     for (int tile = pc.tile_begin; tile < pc.tile_end; ++tile, ++it) {
       const int s = it % C::kStages;
+      // the stage of the tile before this one, which the other warps are likely done with
+      if (!failed && !fetch(it + C::kStages - 1)) failed = true;
       if (!failed && !mbar_wait(full0 + 8 * s, (it / C::kStages) & 1)) failed = true;
       if (failed) continue;
       unsigned char *kt = smem + s * C::kStage + hs * 64, *vt = kt + C::kTile;
@@ -509,13 +590,10 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(A
         __syncwarp();
         wrote = true;
       }
-#pragma unroll 1
-      for (int sub = 0; sub < C::SUBS; ++sub) {
-        const int b16 = 16 * (sub * R + rr);
-        const int n_tok = seq_len - t0 - b16;
-        if (n_tok > 0)
-          st.template step<U, LOG>(kt + b16 * UB, vt + b16 * UB, sc, n_tok, lane, LOG ? lg + static_cast<size_t>(t0 + b16) * g : nullptr, g);
-      }
+      const int n_tok = seq_len - t0 - 16 * rr;
+      if (n_tok > 0)
+        st.template tile<U, LOG>(kt + 16 * rr * UB, vt + 16 * rr * UB, sc, n_tok, lane,
+                                 LOG ? lg + static_cast<size_t>(t0 + 16 * rr) * g : nullptr, g);
       if (wrote) fence_proxy_async();   // before the copy engine refills the stage
       __syncwarp();
       if (lane == 0) mbar_arrive(empty0 + 8 * s);

@@ -5,7 +5,9 @@ libvtensor's C ABI.  Tensors are only unwrapped to pointers and strides here; al
 work happens in the CUDA kernels.  Non-CUDA tensors are rejected: there is no
 CPU path.
 """
+import contextlib
 import ctypes
+import functools
 from ctypes import byref, c_size_t, c_void_p
 
 import torch
@@ -15,12 +17,31 @@ from ._lib import VT_KV_BF16, VT_KV_FP8_E4M3, VT_KV_INT4, check, lib
 _workspaces = {}
 
 
+# Host time per call matters for short sequences (the kernels take a few microseconds), hence: addresses go to ctypes as
+# plain integers, the device is only switched when it is not the current one, sizes that the library computes from
+# shapes alone are remembered.
 def _stream():
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _ptr(t):
-    return c_void_p(t.data_ptr()) if t is not None else c_void_p(0)
+    return t.data_ptr() if t is not None else None
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Context in which ``device`` is the current device."""
+    index = device.index
+    return _SAME_DEVICE if index is None or index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(call, *shape):
+    need = c_size_t()
+    check(getattr(lib, call)(*shape, byref(need)), call)
+    return need.value
 
 
 def _require_cuda(*tensors):
@@ -49,10 +70,8 @@ def kv_row_bytes(num_kv_heads, head_size, kv_cache_dtype="auto"):
 def new_workspace(device, batch, num_heads, head_size, max_seq_len, scored=False):
     """A private, zero-filled scratch buffer for ``decode_step(..., workspace=...)``; ``scored`` adds
     the room that ``scores=`` needs."""
-    need = c_size_t()
-    size = lib.vt_decode_scored_workspace_bytes if scored else lib.vt_decode_attn_workspace_bytes
-    check(size(batch, num_heads, head_size, max_seq_len, byref(need)), "new_workspace")
-    return torch.zeros(need.value, dtype=torch.uint8, device=device)
+    call = "vt_decode_scored_workspace_bytes" if scored else "vt_decode_attn_workspace_bytes"
+    return torch.zeros(_workspace_bytes(call, batch, num_heads, head_size, int(max_seq_len)), dtype=torch.uint8, device=device)
 
 
 def _device_index(device):
@@ -63,10 +82,11 @@ def _scratch(device, nbytes):
     """Scratch cached per device and stream and grown on demand: calls of one stream run back to back, calls of two
     streams may overlap.  While the stream is being captured the buffer belongs to the capture instead: a graph must
     not hold the address of a buffer that a later, larger call replaces, nor share one with another graph."""
-    with torch.cuda.device(device):
+    index = _device_index(device)
+    with _on(device):
         if torch.cuda.is_current_stream_capturing():
             return torch.empty(max(nbytes, 1 << 10), dtype=torch.uint8, device=device)
-        key = (_device_index(device), torch.cuda.current_stream().cuda_stream)
+    key = (index, torch._C._cuda_getCurrentRawStream(index))
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
@@ -77,10 +97,7 @@ def _scratch(device, nbytes):
 def attn_workspace(device, batch, num_heads, head_size, max_seq_len):
     """Scratch for the split-K partials, cached per device and stream and grown on demand.
     One buffer serves every layer because layers run back to back on one stream."""
-    need = c_size_t()
-    check(lib.vt_decode_attn_workspace_bytes(batch, num_heads, head_size, max_seq_len, byref(need)),
-          "vt_decode_attn_workspace_bytes")
-    return _scratch(device, need.value)
+    return _scratch(device, _workspace_bytes("vt_decode_attn_workspace_bytes", batch, num_heads, head_size, int(max_seq_len)))
 
 
 def reshape_and_cache(key, value, key_cache, value_cache, slot_m, slot_mapping, seq_lens, cache_seq_lens,
@@ -101,7 +118,7 @@ def reshape_and_cache(key, value, key_cache, value_cache, slot_m, slot_mapping, 
     if key.stride(2) != 1 or key.stride(1) != head_size or value.stride(2) != 1 or value.stride(1) != head_size:
         raise RuntimeError("reshape_and_cache: key/value rows must be contiguous [kv_heads, head_size]")
     batch = slot_mapping.numel()
-    with torch.cuda.device(key.device):
+    with _on(key.device):
         check(lib.vt_append(_ptr(key), _ptr(value), key.stride(0), value.stride(0), _ptr(key_cache),
                             _ptr(value_cache), _ptr(slot_m), _ptr(slot_mapping), _ptr(seq_lens),
                             _ptr(cache_seq_lens), int(max_seq_len), batch, num_kv_heads, head_size,
@@ -129,7 +146,7 @@ def rotary_embedding_and_cache(positions, query, key, value, head_size, cos_sin_
         raise RuntimeError("rotary_embedding_and_cache: rows must be contiguous")
     if q2.shape[-1] % head_size or k2.shape[-1] != num_kv_heads * head_size or v2.shape[-1] != k2.shape[-1]:
         raise RuntimeError("rotary_embedding_and_cache: inconsistent head counts")
-    with torch.cuda.device(query.device):
+    with _on(query.device):
         check(lib.vt_rope_append(_ptr(positions), _ptr(q2), q2.stride(0), q2.shape[-1] // head_size, _ptr(k2), _ptr(v2),
                                  k2.stride(0), v2.stride(0), _ptr(cos_sin_cache), cos_sin_cache.shape[1],
                                  1 if is_neox else 0, _ptr(key_cache), _ptr(value_cache), _ptr(slot_m),
@@ -148,7 +165,7 @@ def rms_norm(out, input, weight, epsilon):
     x, o = input.view(-1, hidden), out.view(-1, hidden)
     if x.stride(1) != 1 or o.stride(1) != 1:
         raise RuntimeError("rms_norm: rows must be contiguous")
-    with torch.cuda.device(input.device):
+    with _on(input.device):
         check(lib.vt_rms_norm(_ptr(o), _ptr(x), _ptr(weight), float(epsilon), x.shape[0], hidden, x.stride(0),
                               o.stride(0), _stream()), "vt_rms_norm")
 
@@ -162,7 +179,7 @@ def fused_add_rms_norm(input, residual, weight, epsilon):
     if not (input.is_contiguous() and residual.is_contiguous()):
         raise RuntimeError("fused_add_rms_norm: contiguous tensors only")
     hidden = input.shape[-1]
-    with torch.cuda.device(input.device):
+    with _on(input.device):
         check(lib.vt_fused_add_rms_norm(_ptr(input), _ptr(residual), _ptr(weight), float(epsilon),
                                         input.numel() // hidden, hidden, _stream()), "vt_fused_add_rms_norm")
 
@@ -172,7 +189,7 @@ def kv_scales(x, num_kv_heads, head_size):
     _require_cuda(x)
     x = x.view(-1, num_kv_heads, head_size)
     out = torch.empty(num_kv_heads, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         check(lib.vt_kv_scales(_ptr(x), x.stride(0), x.shape[0], num_kv_heads, head_size, _ptr(out), _stream()),
               "vt_kv_scales")
     return out
@@ -192,15 +209,12 @@ def _scored(out, query, key, value, slot_m, k_table, v_table, num_kv_heads, scal
     _check_scores(scores, num_kv_heads, query.device, "scores")
     ws = workspace
     if ws is None:
-        need = c_size_t()
-        check(lib.vt_decode_scored_workspace_bytes(batch, num_heads, head_size, int(max_seq_len), byref(need)),
-              "vt_decode_scored_workspace_bytes")
-        ws = _scratch(query.device, need.value)
-    with torch.cuda.device(query.device):
+        ws = _scratch(query.device, _workspace_bytes("vt_decode_scored_workspace_bytes", batch, num_heads, head_size, int(max_seq_len)))
+    with _on(query.device):
         check(lib.vt_decode_step_scored(_ptr(out), out.stride(0), _ptr(query), query.stride(0), _ptr(key), _ptr(value),
                                         key.stride(0) if key is not None else 0,
-                                        value.stride(0) if value is not None else 0, _ptr(slot_m), c_void_p(int(k_table)),
-                                        c_void_p(int(v_table)), _ptr(slot_ids), _ptr(seq_lens), batch, num_heads,
+                                        value.stride(0) if value is not None else 0, _ptr(slot_m), (int(k_table)),
+                                        (int(v_table)), _ptr(slot_ids), _ptr(seq_lens), batch, num_heads,
                                         num_kv_heads, head_size, int(max_seq_len), float(scale), kv_dtype, _ptr(k_scale),
                                         _ptr(v_scale), _ptr(lse), _ptr(scores), scores.stride(0), scores.stride(1),
                                         scores.shape[2], _ptr(ws), ws.numel(), _stream()), "vt_decode_step_scored")
@@ -212,16 +226,16 @@ def _decode(out, query, k_table, v_table, num_kv_heads, scale, seq_lens, max_seq
     ws = attn_workspace(query.device, batch, num_heads, head_size, max_seq_len)
     if maps is not None and num_splits == 0:
         # plain attention through the tensor-map entry point (no rows to append)
-        with torch.cuda.device(query.device):
+        with _on(query.device):
             check(lib.vt_decode_step_tma(_ptr(out), out.stride(0), _ptr(query), query.stride(0), None, None, 0, 0, None,
-                                         c_void_p(int(k_table)), c_void_p(int(v_table)), _ptr(slot_ids), _ptr(seq_lens),
+                                         (int(k_table)), (int(v_table)), _ptr(slot_ids), _ptr(seq_lens),
                                          batch, num_heads, num_kv_heads, head_size, int(max_seq_len), float(scale),
                                          kv_dtype, _ptr(k_scale), _ptr(v_scale), _ptr(lse), _ptr(ws), ws.numel(), 0,
                                          _ptr(maps), _stream()), "vt_decode_step_tma")
         return
-    with torch.cuda.device(query.device):
-        check(lib.vt_decode_attn(_ptr(out), out.stride(0), _ptr(query), query.stride(0), c_void_p(int(k_table)),
-                                 c_void_p(int(v_table)), _ptr(slot_ids), _ptr(seq_lens), batch, num_heads,
+    with _on(query.device):
+        check(lib.vt_decode_attn(_ptr(out), out.stride(0), _ptr(query), query.stride(0), (int(k_table)),
+                                 (int(v_table)), _ptr(slot_ids), _ptr(seq_lens), batch, num_heads,
                                  num_kv_heads, head_size, int(max_seq_len), float(scale), kv_dtype, _ptr(k_scale),
                                  _ptr(v_scale), _ptr(lse), _ptr(ws), ws.numel(), int(num_splits), _stream()),
               "vt_decode_attn")
@@ -344,18 +358,18 @@ def decode_step(out, query, key, value, key_cache, value_cache, slot_m, slot_map
     if clean_scratch and workspace is None:
         raise RuntimeError("decode_step(clean_scratch=True) needs a private zero-filled workspace")
     if maps is not None:
-        with torch.cuda.device(query.device):
+        with _on(query.device):
             check(lib.vt_decode_step_tma(_ptr(out), out.stride(0), _ptr(query), query.stride(0), _ptr(key), _ptr(value),
-                                         key.stride(0), value.stride(0), _ptr(slot_m), c_void_p(int(key_cache)),
-                                         c_void_p(int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens), batch,
+                                         key.stride(0), value.stride(0), _ptr(slot_m), (int(key_cache)),
+                                         (int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens), batch,
                                          num_heads, num_kv_heads, head_size, int(max_seq_len), float(scale),
                                          _kv_dtype(kv_cache_dtype), _ptr(k_scale), _ptr(v_scale), _ptr(lse), _ptr(ws),
                                          ws.numel(), flags, _ptr(maps), _stream()), "vt_decode_step_tma")
         return
-    with torch.cuda.device(query.device):
+    with _on(query.device):
         check(lib.vt_decode_step(_ptr(out), out.stride(0), _ptr(query), query.stride(0), _ptr(key), _ptr(value),
-                                 key.stride(0), value.stride(0), _ptr(slot_m), c_void_p(int(key_cache)),
-                                 c_void_p(int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens), batch, num_heads,
+                                 key.stride(0), value.stride(0), _ptr(slot_m), (int(key_cache)),
+                                 (int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens), batch, num_heads,
                                  num_kv_heads, head_size, int(max_seq_len), float(scale), _kv_dtype(kv_cache_dtype),
                                  _ptr(k_scale), _ptr(v_scale), _ptr(lse), _ptr(ws), ws.numel(), flags, _stream()),
               "vt_decode_step")
@@ -382,7 +396,7 @@ def prefill_maps(k_bases, v_bases, num_kv_heads, head_size, max_tokens, device):
     vb = (ctypes.c_uint64 * n)(*[int(x) for x in v_bases])
     host = torch.empty(n * 256 + 64, dtype=torch.uint8)
     off = (-host.data_ptr()) % 64
-    with torch.cuda.device(device):
+    with _on(device):
         check(lib.vt_prefill_maps_encode(kb, vb, n, num_kv_heads, head_size, int(max_tokens),
                                          c_void_p(host.data_ptr() + off)), "vt_prefill_maps_encode")
     return host[off: off + n * 256].to(device)
@@ -404,7 +418,7 @@ def decode_maps(k_bases, v_bases, num_kv_heads, head_size, max_tokens, device, k
     vb = (ctypes.c_uint64 * n)(*[int(x) for x in v_bases])
     host = torch.empty(n * 256 + 64, dtype=torch.uint8)
     off = (-host.data_ptr()) % 64
-    with torch.cuda.device(device):
+    with _on(device):
         check(lib.vt_decode_maps_encode(kb, vb, n, num_kv_heads, head_size, _kv_dtype(kv_cache_dtype), int(max_tokens),
                                         c_void_p(host.data_ptr() + off)), "vt_decode_maps_encode")
     return host[off: off + n * 256].to(device)
@@ -436,8 +450,8 @@ def widen_fp8_ranges(key_cache, value_cache, num_kv_heads, head_size, slot_mappi
                           torch.tensor(starts, dtype=torch.int32, device=dev), max(lens) if lens else 0, kv_cache_dtype,
                           k_scale, v_scale)
         return kb, vb, (buf, padded)
-    with torch.cuda.device(dev):
-        check(lib.vt_kv_widen(c_void_p(int(key_cache)), c_void_p(int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens),
+    with _on(dev):
+        check(lib.vt_kv_widen((int(key_cache)), (int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens),
                               len(lens), num_kv_heads, head_size, max(lens) if lens else 0, _ptr(k_scale), _ptr(v_scale),
                               _ptr(kb), _ptr(vb), _stream()), "vt_kv_widen")
     return kb, vb, (buf, padded)
@@ -459,8 +473,8 @@ def dequantize_ranges(key_out, value_out, key_cache, value_cache, num_kv_heads, 
             raise RuntimeError("dequantize_ranges: outputs must be contiguous bfloat16 [rows, kv_heads, head_size]")
     if slot_mapping.dtype != torch.int64 or seq_lens.dtype != torch.int32 or row_start.dtype != torch.int32:
         raise RuntimeError("dequantize_ranges: slot_mapping must be int64, seq_lens and row_start int32")
-    with torch.cuda.device(outs[0].device):
-        check(lib.vt_kv_dequant(c_void_p(int(key_cache)), c_void_p(int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens),
+    with _on(outs[0].device):
+        check(lib.vt_kv_dequant((int(key_cache)), (int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens),
                                 _ptr(row_start), slot_mapping.numel(), num_kv_heads, head_size, int(max_seq_len),
                                 _kv_dtype(kv_cache_dtype), _ptr(k_scale), _ptr(v_scale), _ptr(key_out), _ptr(value_out),
                                 _stream()), "vt_kv_dequant")
@@ -493,11 +507,11 @@ def prefill_attention(out, query, key_cache, value_cache, num_kv_heads, scale, s
         if prefill_tma_supported(num_kv_heads):
             maps = prefill_maps(kb.tolist(), vb.tolist(), num_kv_heads, head_size, max(holder[1]), query.device)
         holder = (holder, kb, vb, slot_mapping, maps)
-    args = (_ptr(out), out.stride(0), _ptr(query), query.stride(0), c_void_p(int(key_cache)),
-            c_void_p(int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens), _ptr(q_lens),
+    args = (_ptr(out), out.stride(0), _ptr(query), query.stride(0), (int(key_cache)),
+            (int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens), _ptr(q_lens),
             _ptr(q_start), slot_mapping.numel(), num_heads, num_kv_heads, head_size,
             int(max_q_len), float(scale), VT_KV_BF16, None)
-    with torch.cuda.device(query.device):
+    with _on(query.device):
         if maps is None:
             check(lib.vt_prefill_attn(*args, _stream()), "vt_prefill_attn")
         else:
@@ -525,7 +539,7 @@ def prompt_scores(scores, query, key_cache, num_kv_heads, scale, slot_mapping, s
     _, num_heads, head_size = query.shape
     batch, max_seq_len = slot_mapping.numel(), int(max_seq_len)
     dtype = _kv_dtype(kv_cache_dtype)
-    step, table, range_ids = max(batch, 1), c_void_p(int(key_cache)), None
+    step, table, range_ids = max(batch, 1), (int(key_cache)), None
     if dtype != VT_KV_BF16:
         if k_scale is None:
             raise RuntimeError(f"prompt_scores: an {kv_cache_dtype} cache needs k_scale")
@@ -536,21 +550,21 @@ def prompt_scores(scores, query, key_cache, num_kv_heads, scale, slot_mapping, s
         bases = range_ids * (max_seq_len * row) + rows.data_ptr()
         starts = (range_ids * max_seq_len).to(torch.int32)
         table = _ptr(bases)
-    need = c_size_t()
     for b in range(0, batch, step):
         n = min(step, batch - b)
-        slots, lens = slot_mapping[b:b + n], seq_lens[b:b + n]
-        check(lib.vt_prompt_scores_workspace_bytes(n, num_heads, num_kv_heads, head_size, max_seq_len, int(window),
-                                                   byref(need)), "vt_prompt_scores_workspace_bytes")
+        slots, lens, qn, qs = slot_mapping, seq_lens, q_lens, q_start
+        if n < batch:
+            slots, lens, qn, qs = (t[b:b + n] for t in (slot_mapping, seq_lens, q_lens, q_start))
+        need = _workspace_bytes("vt_prompt_scores_workspace_bytes", n, num_heads, num_kv_heads, head_size, max_seq_len, int(window))
         if range_ids is not None:
             dequantize_ranges(rows, None, key_cache, 0, num_kv_heads, slots, lens, starts[:n], max_seq_len, kv_cache_dtype,
                               k_scale)
-        ws = _scratch(query.device, need.value + 256)[256:]     # the first word of the scratch is the status word
-        with torch.cuda.device(query.device):
+        ws = _scratch(query.device, need + 256)
+        with _on(query.device):
             check(lib.vt_prompt_scores(_ptr(scores), scores.stride(0), scores.stride(1), scores.shape[2], _ptr(query),
                                        query.stride(0), table, _ptr(slots), _ptr(range_ids), _ptr(lens),
-                                       _ptr(q_lens[b:b + n]), _ptr(q_start[b:b + n]), n, num_heads, num_kv_heads, head_size,
-                                       max_seq_len, int(window), float(scale), _ptr(ws), ws.numel(), _stream()),
+                                       _ptr(qn), _ptr(qs), n, num_heads, num_kv_heads, head_size, max_seq_len, int(window),
+                                       float(scale), ws.data_ptr() + 256, ws.numel() - 256, _stream()),   # a status word leads
                   "vt_prompt_scores")
 
 
@@ -571,13 +585,11 @@ def evict_rows(scores, key_cache, value_cache, num_kv_heads, slot_mapping, seq_l
     if out.shape != scores.shape or out.stride() != scores.stride() or out.dtype != scores.dtype or out.device != scores.device:
         raise RuntimeError("evict_rows: scores_out must be laid out as scores")
     batch, dtype = slot_mapping.numel(), _kv_dtype(kv_cache_dtype)
-    need = c_size_t()
-    check(lib.vt_evict_workspace_bytes(batch, num_kv_heads, int(budget), dtype, byref(need)), "vt_evict_workspace_bytes")
     kept = torch.empty(batch, num_kv_heads, int(budget), dtype=torch.int32, device=scores.device)
-    ws = _scratch(scores.device, need.value)
-    with torch.cuda.device(scores.device):
+    ws = _scratch(scores.device, _workspace_bytes("vt_evict_workspace_bytes", batch, num_kv_heads, int(budget), dtype))
+    with _on(scores.device):
         check(lib.vt_evict_rows(_ptr(scores), _ptr(out), scores.stride(0), scores.stride(1), scores.shape[2],
-                                c_void_p(int(key_cache)), c_void_p(int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens),
+                                (int(key_cache)), (int(value_cache)), _ptr(slot_mapping), _ptr(seq_lens),
                                 batch, num_kv_heads, head_size, int(max_seq_len), int(budget), int(sink), int(recent), dtype,
                                 _ptr(kept), _ptr(ws), ws.numel(), _stream()), "vt_evict_rows")
     return kept
@@ -605,7 +617,7 @@ def workspace_status(workspace):
     """VT_OK (0) unless an attention kernel using this scratch buffer gave up on a
     bounded wait.  Synchronises the current stream."""
     code = ctypes.c_int()
-    with torch.cuda.device(workspace.device):
+    with _on(workspace.device):
         check(lib.vt_decode_attn_status(_ptr(workspace), _stream(), byref(code)), "vt_decode_attn_status")
     return code.value
 

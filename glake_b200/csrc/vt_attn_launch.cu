@@ -501,13 +501,13 @@ int vt_decode_step_scored(void *out, int64_t out_stride, const void *q, int64_t 
 static size_t prompt_scratch(int batch, int kvh, int g, int max_seq_len, int window, int *runs, int *keys) {
   *keys = vt::prompt_run_keys(batch, kvh, max_seq_len);
   *runs = std::max(1, (max_seq_len + *keys - 1) / *keys);
-  return static_cast<size_t>(batch) * kvh * *runs * window * g * sizeof(float2);
+  return 256 + static_cast<size_t>(batch) * kvh * *runs * window * g * sizeof(float2);   // a status word leads
 }
 
 static int prompt_shape(int batch, int h, int kvh, int d, int max_seq_len, int window) {
   if (batch < 0 || h <= 0 || kvh <= 0 || max_seq_len < 0 || window < 1) return VT_ERR_INVALID;
   if (d != vt::kHeadDim || h % kvh != 0) return VT_ERR_UNSUPPORTED;
-  if (static_cast<int64_t>(window) * (h / kvh) > 16384) return VT_ERR_UNSUPPORTED;   // rows kept in shared memory
+  if (static_cast<int64_t>(window) * (h / kvh) > 16384) return VT_ERR_UNSUPPORTED;   // 128 row blocks
   return VT_OK;
 }
 
@@ -516,7 +516,7 @@ int vt_prompt_scores_workspace_bytes(int batch, int h, int kvh, int d, int max_s
   const int st = prompt_shape(batch, h, kvh, d, max_seq_len, window);
   if (st != VT_OK) return st;
   int runs, keys;
-  *bytes = std::max<size_t>(prompt_scratch(batch, kvh, h / kvh, max_seq_len, window, &runs, &keys), 256);
+  *bytes = prompt_scratch(batch, kvh, h / kvh, max_seq_len, window, &runs, &keys);
   return VT_OK;
 }
 
@@ -531,14 +531,14 @@ int vt_prompt_scores(float *scores, int64_t score_slot_stride, int64_t score_hea
   if (batch == 0 || max_seq_len == 0) return VT_OK;
   if (!scores || !q || !k_table || !slot_ids || !seq_lens || !q_lens || !q_start || !workspace) return VT_ERR_INVALID;
   if (max_seq_len > score_rows || score_head_stride < score_rows || score_slot_stride < score_rows) return VT_ERR_INVALID;
-  if ((reinterpret_cast<uintptr_t>(q) & 3) || (q_stride % 2) || q_stride < static_cast<int64_t>(h) * d ||
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || (q_stride % 8) || q_stride < static_cast<int64_t>(h) * d ||
       (reinterpret_cast<uintptr_t>(workspace) & 255))
     return VT_ERR_INVALID;
   int runs, keys;
   if (workspace_bytes < prompt_scratch(batch, kvh, h / kvh, max_seq_len, window, &runs, &keys)) return VT_ERR_INVALID;
   vt::PromptScoreParams p{q, q_stride, k_table, slot_ids, range_ids, seq_lens, q_lens, q_start, batch, h, kvh, max_seq_len,
-                          window, scale, scores, score_slot_stride, score_head_stride, static_cast<float2 *>(workspace),
-                          runs, keys, window * (h / kvh)};
+                          window, scale, scores, score_slot_stride, score_head_stride, reinterpret_cast<float2 *>(static_cast<char *>(workspace) + 256), runs, keys, window * (h / kvh),
+                          static_cast<uint32_t *>(workspace)};
   return vt::launch_prompt_scores(p, static_cast<cudaStream_t>(stream));
 }
 

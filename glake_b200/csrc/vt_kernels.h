@@ -118,6 +118,7 @@ struct PromptScoreParams {
   int64_t slot_stride, head_stride;
   float2 *ml;                         // [batch * kvh, runs, rows]: (maximum in the log2 domain, sum) of a run
   int runs, run_keys, rows;           // rows = window * (h / kvh)
+  uint32_t *status;
 };
 int launch_prompt_scores(const PromptScoreParams &p, cudaStream_t stream);
 int prompt_run_keys(int batch, int kvh, int max_seq_len);

@@ -559,13 +559,12 @@ def prompt_scores(scores, query, key_cache, num_kv_heads, scale, slot_mapping, s
         if range_ids is not None:
             dequantize_ranges(rows, None, key_cache, 0, num_kv_heads, slots, lens, starts[:n], max_seq_len, kv_cache_dtype,
                               k_scale)
-        ws = _scratch(query.device, need + 256)
+        ws = _scratch(query.device, need)
         with _on(query.device):
             check(lib.vt_prompt_scores(_ptr(scores), scores.stride(0), scores.stride(1), scores.shape[2], _ptr(query),
                                        query.stride(0), table, _ptr(slots), _ptr(range_ids), _ptr(lens),
                                        _ptr(qn), _ptr(qs), n, num_heads, num_kv_heads, head_size, max_seq_len, int(window),
-                                       float(scale), ws.data_ptr() + 256, ws.numel() - 256, _stream()),   # a status word leads
-                  "vt_prompt_scores")
+                                       float(scale), _ptr(ws), ws.numel(), _stream()), "vt_prompt_scores")
 
 
 def evict_rows(scores, key_cache, value_cache, num_kv_heads, slot_mapping, seq_lens, max_seq_len, budget, sink=0, recent=0,

@@ -374,11 +374,12 @@ int vt_decode_step_scored(void *out, int64_t out_stride, const void *q, int64_t 
  * vt_decode_step_scored): with w = min(window, q_lens[i], seq_lens[i]), the last w of entry i's new
  * tokens, query j of them seeing rows 0 .. seq_lens[i] - w + j, each add their softmax weights,
  * summed over the q heads of a kv head.
- *   q           bf16 [tokens, h, d], row stride in elements (even), 4-byte aligned; q_lens / q_start as
- *               in vt_prefill_attn
+ *   q           bf16 [tokens, h, d], 16-byte aligned, row stride a multiple of 8 elements; q_lens /
+ *               q_start as in vt_prefill_attn
  *   k_table     bf16 ranges; range_ids (device int64 [batch]) index it, NULL = slot_ids.  A quantised
  *               cache is read back first (vt_kv_dequant) and named through range_ids
- *   workspace   vt_prompt_scores_workspace_bytes, 256-byte aligned, content irrelevant
+ *   workspace   vt_prompt_scores_workspace_bytes, 256-byte aligned, content irrelevant; its first word
+ *               reads as vt_decode_attn_status says
  * max_seq_len bounds seq_lens (a longer context is cut there) and is at most score_rows;
  * window * h / kvh <= 16384.  No counterpart in the reference. */
 int vt_prompt_scores_workspace_bytes(int batch, int h, int kvh, int d, int max_seq_len, int window, size_t *bytes);

@@ -61,7 +61,7 @@ __device__ __forceinline__ float ex2(float x) {
 
 // fragment row -> token of the warp's 16 (see the header: conflict-free at the pitch of U heads)
 template <int U>
-__device__ __forceinline__ int token_of_row(int row) {
+__host__ __device__ constexpr int token_of_row(int row) {
   const int i = row & 7;
   if (U == 8)    // pitch 136 words = 8 mod 32
     return static_cast<int>((0x53427160u >> (4 * i)) & 15u) + (row & 8);
@@ -79,8 +79,6 @@ __device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[
 template <int NB>
 struct WarpAttn4 {
   uint32_t qb[NB][4][2][2];   // [group][step][k half]
-  float qoff[NB][4][2];       // -8 sum q over the group, per column
-  float qmul[NB][2];          // partial logits -> log2 domain
   float o[NB][8][4];
   float corr[NB][4];          // row G: 8 sum p s_v[G]
   float mrun[NB][2], lrun[NB][2];
@@ -89,7 +87,12 @@ struct WarpAttn4 {
     return 32 * (mb >> 1) + 4 * r4 + 2 * (mb & 1) + half;
   }
 
-  __device__ __forceinline__ void start(const __nv_bfloat16 *qrow, int g, float sl2, int lane) {
+  // Per q head of the warp, in shared memory (ten registers the tile loop would spill): -8 sum q of every group, and the
+  // factor from partial logits to the log2 domain.
+  static constexpr int kQRow = 6;   // floats: 4 offsets, factor, pad
+  static constexpr int kQFloats = NB * 8 * kQRow;
+
+  __device__ __forceinline__ void start(const __nv_bfloat16 *qrow, int g, float sl2, int lane, float *qs) {
     const int r4 = lane >> 2, c4 = lane & 3;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -127,13 +130,14 @@ struct WarpAttn4 {
         sum[G] += __shfl_xor_sync(0xffffffffu, sum[G], 1);
         sum[G] += __shfl_xor_sync(0xffffffffu, sum[G], 2);
       }
-      const float mul = sl2 * (16777216.f / f);   // 2^24 of the nibbles, 1 / f of Q
+      if (c4 == 0) {
+        float *mine = qs + head * kQRow;
+#pragma unroll
+        for (int G = 0; G < 4; ++G) mine[G] = sum[G] * -4.76837158203125e-7f;   // -8 2^-24
+        mine[4] = sl2 * (16777216.f / f);   // 2^24 of the nibbles, 1 / f of Q
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int src = (2 * c4 + e) * 4;
-#pragma unroll
-        for (int G = 0; G < 4; ++G) qoff[nb][G][e] = __shfl_sync(0xffffffffu, sum[G], src) * -4.76837158203125e-7f;   // -8 2^-24
-        qmul[nb][e] = __shfl_sync(0xffffffffu, mul, src);
         mrun[nb][e] = -INFINITY;
         lrun[nb][e] = 0.f;
       }
@@ -141,17 +145,18 @@ struct WarpAttn4 {
       for (int mb = 0; mb < 8; ++mb) o[nb][mb][0] = o[nb][mb][1] = o[nb][mb][2] = o[nb][mb][3] = 0.f;
       corr[nb][0] = corr[nb][1] = corr[nb][2] = corr[nb][3] = 0.f;
     }
+    __syncwarp();
   }
 
   // Partial logits of 16 tokens per group of dims, joined with the group scales: s[nb][token ta: heads 2 c4, + 1; tb: ..].
   template <int U>
-  __device__ __forceinline__ void logits(float (&s)[NB][4], const unsigned char *kt, int sc, int ta, int tb, int c4) const {
-    constexpr int UB = Cfg4<U>::UB;
+  __device__ __forceinline__ void logits(float (&s)[NB][4], const unsigned char *kt, int sc, const int4 &at, int c4, const float *qs) const {
+    constexpr int DB = Cfg4<U>::UB * token_of_row<U>(8);   // from fragment row r4 to r4 + 8
     float acc[NB][4][4];
-    const uint4 ka = *reinterpret_cast<const uint4 *>(kt + ta * UB + 16 * c4);
-    const uint4 kb = *reinterpret_cast<const uint4 *>(kt + tb * UB + 16 * c4);
-    const uint32_t wsa = *reinterpret_cast<const uint32_t *>(kt + ta * UB + sc);
-    const uint32_t wsb = *reinterpret_cast<const uint32_t *>(kt + tb * UB + sc);
+    const uint4 ka = *reinterpret_cast<const uint4 *>(kt + at.x);
+    const uint4 kb = *reinterpret_cast<const uint4 *>(kt + at.x + DB);
+    const uint32_t wsa = *reinterpret_cast<const uint32_t *>(kt + at.y + sc);
+    const uint32_t wsb = *reinterpret_cast<const uint32_t *>(kt + at.y + DB + sc);
 #pragma unroll
     for (int G = 0; G < 4; ++G) {
       const uint32_t sel = (G & 1) ? 0x7632u : 0x5410u;
@@ -177,37 +182,40 @@ struct WarpAttn4 {
     for (int nb = 0; nb < NB; ++nb) {
       // the "- 8" of a group is added to its sum here, on the FMA pipe: as the start value of the accumulators it
       // costs a move per register on the ALU pipe, which is the busy one
+      const float *q0 = qs + (nb * 8 + 2 * c4) * kQRow, *q1 = q0 + kQRow;
 #pragma unroll
       for (int G = 0; G < 4; ++G) {
-        const float x0 = acc[nb][G][0] + qoff[nb][G][0], x1 = acc[nb][G][1] + qoff[nb][G][1];
-        const float x2 = acc[nb][G][2] + qoff[nb][G][0], x3 = acc[nb][G][3] + qoff[nb][G][1];
+        const float x0 = acc[nb][G][0] + q0[G], x1 = acc[nb][G][1] + q1[G];
+        const float x2 = acc[nb][G][2] + q0[G], x3 = acc[nb][G][3] + q1[G];
         s[nb][0] = G ? fmaf(ga[G], x0, s[nb][0]) : ga[G] * x0;
         s[nb][1] = G ? fmaf(ga[G], x1, s[nb][1]) : ga[G] * x1;
         s[nb][2] = G ? fmaf(gb[G], x2, s[nb][2]) : gb[G] * x2;
         s[nb][3] = G ? fmaf(gb[G], x3, s[nb][3]) : gb[G] * x3;
       }
+      s[nb][0] *= q0[4]; s[nb][1] *= q1[4];
+      s[nb][2] *= q0[4]; s[nb][3] *= q1[4];
     }
   }
 
   // O^T += V^T . (s_v P)^T over 16 tokens; pb = P^T as a B operand.
   template <int U>
-  __device__ __forceinline__ void values(const uint32_t (&pb)[NB][2], const unsigned char *vt, int sc, int n_tok, int r4, int c4) {
-    constexpr int UB = Cfg4<U>::UB;
-    const int t0 = token_of_row<U>(2 * c4), t1 = token_of_row<U>(2 * c4 + 1);
-    const int t2 = token_of_row<U>(2 * c4 + 8), t3 = token_of_row<U>(2 * c4 + 9);
-    const uint2 v0 = *reinterpret_cast<const uint2 *>(vt + t0 * UB + 8 * r4);
-    const uint2 v1 = *reinterpret_cast<const uint2 *>(vt + t1 * UB + 8 * r4);
-    const uint2 v2 = *reinterpret_cast<const uint2 *>(vt + t2 * UB + 8 * r4);
-    const uint2 v3 = *reinterpret_cast<const uint2 *>(vt + t3 * UB + 8 * r4);
-    uint32_t w0 = *reinterpret_cast<const uint32_t *>(vt + t0 * UB + sc);
-    uint32_t w1 = *reinterpret_cast<const uint32_t *>(vt + t1 * UB + sc);
-    uint32_t w2 = *reinterpret_cast<const uint32_t *>(vt + t2 * UB + sc);
-    uint32_t w3 = *reinterpret_cast<const uint32_t *>(vt + t3 * UB + sc);
+  __device__ __forceinline__ void values(const uint32_t (&pb)[NB][2], const unsigned char *vt, int sc, int n_tok, const int4 &at, int r4) {
+    constexpr int UB = Cfg4<U>::UB, DB = UB * token_of_row<U>(8);
+    const int o0 = at.z, o1 = at.w;
+    const uint2 v0 = *reinterpret_cast<const uint2 *>(vt + o0 + 8 * r4);
+    const uint2 v1 = *reinterpret_cast<const uint2 *>(vt + o1 + 8 * r4);
+    const uint2 v2 = *reinterpret_cast<const uint2 *>(vt + o0 + DB + 8 * r4);
+    const uint2 v3 = *reinterpret_cast<const uint2 *>(vt + o1 + DB + 8 * r4);
+    uint32_t w0 = *reinterpret_cast<const uint32_t *>(vt + o0 + sc);
+    uint32_t w1 = *reinterpret_cast<const uint32_t *>(vt + o1 + sc);
+    uint32_t w2 = *reinterpret_cast<const uint32_t *>(vt + o0 + DB + sc);
+    uint32_t w3 = *reinterpret_cast<const uint32_t *>(vt + o1 + DB + sc);
     if (n_tok < 16) {   // what lies past the context is stale and may be NaN as a scale; its P is 0
-      w0 = t0 < n_tok ? w0 : 0u;
-      w1 = t1 < n_tok ? w1 : 0u;
-      w2 = t2 < n_tok ? w2 : 0u;
-      w3 = t3 < n_tok ? w3 : 0u;
+      const int end = n_tok * UB;
+      w0 = o0 < end ? w0 : 0u;
+      w1 = o1 < end ? w1 : 0u;
+      w2 = o0 + DB < end ? w2 : 0u;
+      w3 = o1 + DB < end ? w3 : 0u;
     }
     // per pair of tokens the scale bytes of groups (0, 1) and (2, 3), interleaved
     const uint32_t y01[2] = {prmt(w0, w1, 0x5140u), prmt(w0, w1, 0x7362u)};
@@ -245,14 +253,13 @@ struct WarpAttn4 {
   // One tile of this warp: SUBS x 16 tokens, `stride` tokens apart.  kt / vt = the head's K / V bytes of the first
   // token, sc = offset of the scale words from there, n_tok > 0 = tokens from that one to the end of the context.
   template <int U, bool LOG>
-  __device__ __forceinline__ void tile(const unsigned char *kt, const unsigned char *vt, int sc, int n_tok, int lane, float *lg,
+  __device__ __forceinline__ void tile(const unsigned char *kt, const unsigned char *vt, int sc, int n_tok, int lane, const float *qs, const int4 &at, float *lg,
                                        int g) {
     constexpr int SUBS = Cfg4<U>::SUBS, STEP = 16 * Cfg4<U>::R, UB = Cfg4<U>::UB;
     const int r4 = lane >> 2, c4 = lane & 3;
-    const int ta = token_of_row<U>(r4), tb = token_of_row<U>(r4 + 8);
     float s[SUBS][NB][4];
 #pragma unroll
-    for (int i = 0; i < SUBS; ++i) logits<U>(s[i], kt + i * STEP * UB, sc, ta, tb, c4);
+    for (int i = 0; i < SUBS; ++i) logits<U>(s[i], kt + i * STEP * UB, sc, at, c4, qs);
     // ---- online softmax (rows = tokens ta, tb; columns = heads 2 c4, 2 c4 + 1) ----
     uint32_t pb[SUBS][NB][2];
     float fac[NB][2];
@@ -263,12 +270,11 @@ struct WarpAttn4 {
 #pragma unroll
       for (int i = 0; i < SUBS; ++i) {
         float(&x)[4] = s[i][nb];
-        x[0] *= qmul[nb][0];
-        x[1] *= qmul[nb][1];
-        x[2] *= qmul[nb][0];
-        x[3] *= qmul[nb][1];
+        const bool ragged = n_tok < (SUBS - 1) * STEP + 16;   // the context ends in this tile
+        int ta = 0, tb = 0;
+        if (LOG || ragged) { ta = at.y / UB; tb = ta + token_of_row<U>(8); }
         const bool va = ta + i * STEP < n_tok, vb = tb + i * STEP < n_tok;
-        if (n_tok < (SUBS - 1) * STEP + 16) {   // the context ends in this tile
+        if (ragged) {
           x[0] = va ? x[0] : -INFINITY;
           x[1] = va ? x[1] : -INFINITY;
           x[2] = vb ? x[2] : -INFINITY;
@@ -324,7 +330,7 @@ struct WarpAttn4 {
       }
     }
 #pragma unroll
-    for (int i = 0; i < SUBS; ++i) values<U>(pb[i], vt + i * STEP * UB, sc, n_tok - i * STEP, r4, c4);
+    for (int i = 0; i < SUBS; ++i) values<U>(pb[i], vt + i * STEP * UB, sc, n_tok - i * STEP, at, r4);
   }
 
   // Row sums over the lanes, the "- 8" correction and the powers of two: afterwards o and lrun are what the
@@ -378,283 +384,430 @@ struct WarpAttn4 {
   }
 };
 
-// Where a warp's copies stand: the tile to fetch next.  In shared memory: it is needed once per tile, registers always.
-struct Cursor {
-  const char *k, *v;         // the unit's rows of the piece's sequence
-  long long tau;             // position of the piece after this one
-  int tile, tile_end, seq_len, pad;
+// What a warp keeps in shared memory, because registers held over the tile loop are the scarce resource (spills go to
+// an L1 that the rings leave 20 KB of: a handful of reloads per tile cost 200 of 440 us): the pieces of its share ahead
+// of it and where its copies stand.
+struct PieceRec {
+  const char *k, *v;               // the unit's rows of the piece's sequence
+  int b, slab, tile_begin, tile_end, tiles, seq_len;   // as Piece; tiles = of the whole stream
+  int stream_begin, stream_end;
+};
+constexpr int kPieces = 4;         // the copies run at most two tiles ahead, so they stay within the next three pieces
+struct alignas(16) WarpState {
+  PieceRec piece[kPieces];
+  int tau, pieces;                 // position after, and number of, the pieces looked up so far
+  int copy_piece, copy_tile;       // next tile to fetch
+  uint32_t fresh[2][32];           // fused step: the lanes' 16 bits and scale byte (<< 16) of the newest K and V row
 };
 
-// ring | barriers | cursors | flags | prefix[batch + 1] | lens[batch] | (pad to 8) | kbase[batch] | vbase[batch]
+// ring | barriers | warp states | q statistics | flags | prefix[batch + 1] | lens[batch] | (pad to 8) | kbase[batch] | vbase[batch]
 __host__ __device__ constexpr int meta_ints4(int batch) { return ((2 * batch + 1 + 4) + 1) / 2 * 2; }
+template <int U, int NB>
+struct Layout4 {
+  static constexpr int kBars = Cfg4<U>::kStages * Cfg4<U>::kStage;
+  static constexpr int kWarp = kBars + Cfg4<U>::kStages * 16;
+  static constexpr int kQ = kWarp + kCWarps * static_cast<int>(sizeof(WarpState));
+  static constexpr int kAt = kQ + kCWarps * WarpAttn4<NB>::kQFloats * 4;      // per lane: fragment offsets in a tile
+  static constexpr int kMeta = kAt + 32 * 16;   // 4 ints: total positions, CTAs, end of the share
+  static constexpr int bytes(int batch) { return kMeta + meta_ints4(batch) * 4 + (batch <= kBaseCacheMaxBatch4 ? batch * 16 : 0); }
+  static_assert(sizeof(WarpState) % 8 == 0 && kQ % 8 == 0 && kAt % 16 == 0 && kMeta % 8 == 0, "alignment");
+};
+
+// Merge of one kv head of a stream by the warp that drew its last ticket (scratch layout of merge_stream, but a ticket
+// counter per head and no meeting of the CTA's warps: the heads of a stream are then merged by whichever CTAs finish
+// last, side by side; one CTA doing all of them took 12 of a 21 us call over 700 rows of 32/8 heads, its reads of
+// 370 KB alone).  Four q heads at a time with sixteen 16-byte rows in flight, the first before the weights are known.
+template <int U, int R, int HEADS>
+__device__ __noinline__ void merge_head(const AttnParams &p, int b, int kv_head, int stream_begin, long long total, int n_ctas,
+                                        int c_first, int c_last, int lane, int g) {
+  constexpr int I = 4, J = 4;
+  const int n_src = (c_last - c_first + 1) * R, hh = kv_head % U;
+  const int slot0 = stream_begin <= total * c_first / n_ctas ? 0 : 1;   // later CTAs start inside the stream: slot 0
+  const auto row = [&](int i, int head) -> const float * {
+    const int c = i / R, r = i % R;
+    const size_t slot = static_cast<size_t>(c_first + c) * 2 + (c == 0 ? slot0 : 0);
+    return p.fl_part + ((slot * kCWarps + r * U + hh) * HEADS + head) * kPartRow;
+  };
+  const float vsc = __ldg(p.v_scale + kv_head);
+  for (int h0 = 0; h0 < g; h0 += I) {
+    float M[I], L[I];
+    float4 acc[I];
+#pragma unroll
+    for (int k = 0; k < I; ++k) {
+      M[k] = -INFINITY;
+      L[k] = 0.f;
+      acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const int n_heads = min(I, g - h0);
+    for (int s0 = 0; s0 < n_src; s0 += 32) {
+      const int cnt = min(32, n_src - s0);
+      float2 ml[I];
+#pragma unroll
+      for (int k = 0; k < I; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+        if (lane < cnt && k < n_heads) ml[k] = __ldcg(reinterpret_cast<const float2 *>(row(s0 + lane, h0 + k) + 128));
+      }
+      float4 v[J][I];
+      const auto fetch = [&](int j0) {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int k = 0; k < I; ++k) {
+            v[j][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < n_heads && j0 + j < cnt) v[j][k] = __ldcg(reinterpret_cast<const float4 *>(row(s0 + j0 + j, h0 + k)) + lane);
+          }
+      };
+      fetch(0);
+      float w[I];   // weight of source s0 + lane
+#pragma unroll
+      for (int k = 0; k < I; ++k) {
+        float mx = ml[k].x;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float Mn = fmaxf(M[k], mx), f = M[k] == -INFINITY ? 0.f : ex2(M[k] - Mn);
+        w[k] = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - Mn);
+        float sum = w[k] * ml[k].y;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        L[k] = L[k] * f + sum;
+        acc[k].x *= f; acc[k].y *= f; acc[k].z *= f; acc[k].w *= f;
+        M[k] = Mn;
+      }
+      for (int j0 = 0; j0 < cnt; j0 += J) {
+        if (j0 > 0) fetch(j0);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int k = 0; k < I; ++k) {
+            const float y = __shfl_sync(0xffffffffu, w[k], (j0 + j) & 31);   // 0 behind the last source
+            acc[k].x = fmaf(y, v[j][k].x, acc[k].x); acc[k].y = fmaf(y, v[j][k].y, acc[k].y);
+            acc[k].z = fmaf(y, v[j][k].z, acc[k].z); acc[k].w = fmaf(y, v[j][k].w, acc[k].w);
+          }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < I; ++k) {
+      if (k < n_heads) {
+        const int hq = kv_head * g + h0 + k;
+        const float inv = vsc / L[k];
+        uint2 packed;
+        packed.x = pack_bf16(acc[k].x * inv, acc[k].y * inv);
+        packed.y = pack_bf16(acc[k].z * inv, acc[k].w * inv);
+        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + b * p.out_stride + hq * kHeadDim + lane * 4) = packed;
+        if (lane == 0) write_stats(p, b * p.h + hq, M[k], L[k]);
+      }
+    }
+  }
+}
+
+// Looks up pieces of the share until kPieces - 1 lie ahead of piece `now`, or the share ends.  meta: the CTA's flags.
+template <int UB>
+__device__ __noinline__ void look_ahead(const AttnParams &p, WarpState &ws, const int *meta, int slabs, int now, int lane) {
+  const int *prefix = meta + 4, *lens = prefix + p.batch + 1;
+  const unsigned long long *bases = reinterpret_cast<const unsigned long long *>(meta + meta_ints4(p.batch));
+  int tau = ws.tau, n = ws.pieces;
+  const int end = meta[2];
+  __syncwarp();
+  while (tau < end && n < now + kPieces) {
+    const Piece pc = locate(prefix, p.batch, slabs, tau, end);
+    tau += pc.advance;
+    if (pc.tile_end <= pc.tile_begin) continue;   // only phantom positions of this stream fall into the share
+    if (lane == 0) {
+      PieceRec &r = ws.piece[n % kPieces];
+      const bool cached = p.batch <= kBaseCacheMaxBatch4;
+      const int64_t slot = cached ? 0 : p.slot_ids[pc.b];
+      r.k = reinterpret_cast<const char *>(cached ? bases[pc.b] : p.k_table[slot]) + pc.slab * UB;
+      r.v = reinterpret_cast<const char *>(cached ? bases[p.batch + pc.b] : p.v_table[slot]) + pc.slab * UB;
+      r.b = pc.b; r.slab = pc.slab; r.tile_begin = pc.tile_begin; r.tile_end = pc.tile_end; r.tiles = pc.tiles_in_stream;
+      r.seq_len = lens[pc.b];
+      r.stream_begin = static_cast<int>(pc.stream_begin); r.stream_end = static_cast<int>(pc.stream_end);
+    }
+    ++n;
+  }
+  if (lane == 0) { ws.tau = tau; ws.pieces = n; }
+  __syncwarp();
+}
+
+// Fused step: quantises the step's row of this warp's head, stores it into the ranges and leaves the lanes' bits in ws.
 template <int U>
-constexpr int smem_bytes4(int batch) {
-  return Cfg4<U>::kStages * (Cfg4<U>::kStage + 16) + kCWarps * static_cast<int>(sizeof(Cursor)) + meta_ints4(batch) * 4 + (batch <= kBaseCacheMaxBatch4 ? batch * 16 : 0);
+__device__ __noinline__ void append_row(const AttnParams &p, WarpState &ws, const PieceRec &pc, int hs, int64_t off, int lane) {
+  const int kv_head = pc.slab * U + hs, at = 8 * (lane & 7) + 2 * (lane >> 3);
+  for (int kv = 0; kv < 2; ++kv) {
+    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(kv ? p.new_value : p.new_key) +
+                               pc.b * (kv ? p.new_value_stride : p.new_key_stride) + kv_head * kHeadDim + lane * 4;
+    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(src));
+    const float x[4] = {bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
+    uint32_t bits, s8;
+    quantise4(x, (kv ? p.v_scale : p.k_scale)[kv_head], &bits, &s8);
+    char *far = const_cast<char *>(kv ? pc.v : pc.k) + off;   // the unit's bytes of the row
+    *reinterpret_cast<uint16_t *>(far + hs * 64 + at) = static_cast<uint16_t>(bits);
+    if ((lane & 7) == 0) far[U * 64 + hs * 4 + (lane >> 3)] = static_cast<char>(s8);
+    ws.fresh[kv][lane] = bits | s8 << 16;
+  }
+  __syncwarp();
+}
+
+// Every warp fetches an eighth of the rows of the CTA's next tile into its ring stage, `n` tiles into the share, once all
+// warps are done with what the stage held; false when a bounded wait ran out.  A single-unit cache is contiguous over
+// tokens: one copy of K and one of V.  Otherwise a row of the unit (80 to 544 bytes) is one copy, a lane each.
+template <int U>
+__device__ __forceinline__ bool fetch_tile(const AttnParams &p, unsigned char *smem, WarpState &ws, int n, int slabs, int warp, int lane) {
+  using C = Cfg4<U>;
+  constexpr int UB = C::UB, ROWS = C::TOK / kCWarps;
+  static_assert(ROWS <= 16, "a lane per row of K and of V");
+  int piece = ws.copy_piece, tile = ws.copy_tile;
+  if (piece >= ws.pieces) return true;   // the share is fetched
+  const PieceRec &pc = ws.piece[piece % kPieces];
+  const int s = n % C::kStages;
+  const int t0 = tile * C::TOK + warp * ROWS, nt = min(max(pc.seq_len - t0, 0), ROWS);
+  const int64_t src = static_cast<int64_t>(t0) * (slabs * UB);
+  const char *kb = pc.k + src, *vb = pc.v + src;
+  ++tile;
+  if (tile >= pc.tile_end) {
+    ++piece;
+    tile = ws.piece[piece % kPieces].tile_begin;
+  }
+  const uint32_t bar = smem_u32(smem) + C::kStages * C::kStage + 8 * s;   // full; the empty ones follow
+  if (n >= C::kStages && !mbar_wait(bar + 8 * C::kStages, ((n / C::kStages) - 1) & 1)) {
+    if (lane == 0) atomicExch(p.status, kKernelErrMagic);
+    return false;
+  }
+  const uint32_t dst = smem_u32(smem) + s * C::kStage + warp * ROWS * UB;
+  __syncwarp();
+  if (lane == 0) {
+    ws.copy_piece = piece;
+    ws.copy_tile = tile;
+    mbar_arrive_expect_tx(bar, 2u * nt * UB);
+  }
+  __syncwarp();
+  const uint64_t policy = l2_policy_evict_first();
+  if (slabs == 1) {
+    if (lane < 2 && nt > 0) bulk_g2s_hint(dst + lane * C::kTile, lane ? vb : kb, nt * UB, bar, policy);
+  } else {
+    const int row = lane & 15;
+    if (row < nt)
+      bulk_g2s_hint(dst + (lane >> 4) * C::kTile + row * UB, (lane >> 4 ? vb : kb) + static_cast<int64_t>(row) * (slabs * UB), UB, bar,
+                    policy);
+  }
+  return true;
+}
+
+// Piece `now` of the CTA's share, the `it`-th tile on: attention, then either the result or a published state and a
+// ticket.  Bit 0: a bounded wait ran out; bit 1: this warp drew the last ticket of its head.  A function of its own, with
+// no calls inside: what the compiler would otherwise keep on the stack across the merge it reloads in the tile loop.
+template <int U, int NB, bool LOG>
+__device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, bool failed, bool fresh) {
+  using C = Cfg4<U>;
+  using S = Layout4<U, NB>;
+  constexpr int R = C::R, UB = C::UB, TOK = C::TOK, HEADS = NB * 8;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hs = warp % U, rr = warp / U;      // head of the unit, token sub-row
+  WarpState &ws = reinterpret_cast<WarpState *>(smem + S::kWarp)[warp];
+  float *qs = reinterpret_cast<float *>(smem + S::kQ) + warp * WarpAttn4<NB>::kQFloats;
+  const int *meta = reinterpret_cast<const int *>(smem + S::kMeta);
+  const uint32_t full0 = smem_u32(smem + S::kBars), empty0 = full0 + 8 * C::kStages;
+  const int g = p.h / p.kvh, slabs = p.kvh / U;
+  const PieceRec &pc = ws.piece[now % kPieces];
+  WarpAttn4<NB> st;
+  {
+    const int kv_head = pc.slab * U + hs;
+    st.start(static_cast<const __nv_bfloat16 *>(p.q) + pc.b * p.q_stride + kv_head * g * kHeadDim, g,
+             p.scale * 1.4426950408889634f * p.k_scale[kv_head], lane, qs);
+  }
+  int left = pc.seq_len - pc.tile_begin * TOK;   // tokens from the tile's first to the end of the context
+  for (int tiles = pc.tile_end - pc.tile_begin; tiles > 0; --tiles, ++it, left -= TOK) {
+    const int s = it % C::kStages;
+    // the stage of the tile before this one, which the other warps are likely done with
+    if (!failed && !fetch_tile<U>(p, smem, ws, it + C::kStages - 1, slabs, warp, lane)) failed = true;
+    if (!failed && !mbar_wait(full0 + 8 * s, (it / C::kStages) & 1)) failed = true;
+    if (failed) continue;
+    unsigned char *kt = smem + s * C::kStage + hs * 64;
+    constexpr int kSc = U * 64;   // scale words from the unit's first byte
+    const bool overlay = fresh && left <= TOK;
+    if (overlay) {   // the copy brought whatever the range held in the newest row's place
+      const int at = 8 * (lane & 7) + 2 * (lane >> 3);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t w = ws.fresh[kv][lane];
+        unsigned char *row = kt + kv * C::kTile + (left - 1) * UB;
+        *reinterpret_cast<uint16_t *>(row + at) = static_cast<uint16_t>(w);
+        if ((lane & 7) == 0) row[kSc - hs * 60 + (lane >> 3)] = static_cast<unsigned char>(w >> 16);
+      }
+      __syncwarp();
+    }
+    const int n_tok = left - 16 * rr;
+    if (n_tok > 0) {
+      float *lg = nullptr;
+      if constexpr (LOG)
+        lg = p.logits + ((static_cast<size_t>(pc.b) * p.kvh + pc.slab * U + hs) * p.logit_rows + (pc.seq_len - n_tok)) * g;
+      st.template tile<U, LOG>(kt + 16 * rr * UB, kt + C::kTile + 16 * rr * UB, kSc - hs * 60, n_tok, lane, qs,
+                               reinterpret_cast<const int4 *>(smem + S::kAt)[lane], lg, g);
+    }
+    if (overlay) fence_proxy_async();   // before the copy engine refills the stage
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty0 + 8 * s);
+  }
+  st.finish(lane);
+
+  const int kv_head = pc.slab * U + hs;
+  const bool whole = pc.tile_begin == 0 && pc.tile_end == pc.tiles;
+  if (R == 1 && whole) {
+    const int r4 = lane >> 2, c4 = lane & 3;
+    const float vs = p.v_scale[kv_head];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int head = nb * 8 + 2 * c4 + e;
+        if (head < g) {
+          const float inv = vs / st.lrun[nb][e];
+          const int hq = kv_head * g + head;
+          __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(p.out) + pc.b * p.out_stride + hq * kHeadDim;
+#pragma unroll
+          for (int mb = 0; mb < 8; ++mb)   // dims d, d + 1 are the two fragment rows
+            *reinterpret_cast<uint32_t *>(dst + WarpAttn4<NB>::dim_of(mb, 0, r4)) =
+                pack_bf16(st.o[nb][mb][e] * inv, st.o[nb][mb][2 + e] * inv);
+          if (r4 == 0) write_stats(p, pc.b * p.h + hq, st.mrun[nb][e], st.lrun[nb][e]);
+        }
+      }
+    }
+  } else {
+    if (p.overlap) pdl_wait_prior_grid();   // the scratch is shared with the previous launch
+    float *slot_base = p.fl_part + (static_cast<size_t>(blockIdx.x) * 2 + (now == 0 ? 0 : 1)) * kCWarps * HEADS * kPartRow;
+    st.template store<kPartRow>(slot_base + warp * HEADS * kPartRow, lane, g);
+    const long long total = meta[0];
+    const int n_ctas = meta[1];
+    const int c_first = owner_of(pc.stream_begin + kBoundaryCost, total, n_ctas);
+    const int c_last = owner_of(pc.stream_end - 1, total, n_ctas);
+    __syncwarp();
+    int last = 0;
+    if (lane == 0) {   // one ticket per warp; the fence covers the stores of the lanes it has met
+      __threadfence();
+      unsigned *ctr = p.fl_count + pc.b * p.kvh + kv_head;
+      last = atomicAdd(ctr, 1u) + 1 == static_cast<unsigned>((c_last - c_first + 1) * R);
+      if (last) *ctr = 0u;   // clean for the next launch
+      __threadfence();
+    }
+    return (failed ? 1 : 0) | (__shfl_sync(0xffffffffu, last, 0) << 1);
+  }
+  return failed ? 1 : 0;
 }
 
 template <int U, int NB, bool LOG>
-__global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(AttnParams p) {
+__global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(const __grid_constant__ AttnParams p) {
   using C = Cfg4<U>;
+  using S = Layout4<U, NB>;
   constexpr int R = C::R, UB = C::UB, TOK = C::TOK, HEADS = NB * 8;
   extern __shared__ __align__(128) unsigned char smem[];
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kStages * C::kStage);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Cursor &cur = reinterpret_cast<Cursor *>(bars + 2 * C::kStages)[warp];
-  int *flags = reinterpret_cast<int *>(reinterpret_cast<Cursor *>(bars + 2 * C::kStages) + kCWarps);
-  int *prefix = flags + 4;
-  int *lens = prefix + p.batch + 1;
-  const bool cache_bases = p.batch <= kBaseCacheMaxBatch4;
-  unsigned long long *kbase_s = reinterpret_cast<unsigned long long *>(flags + meta_ints4(p.batch));
-  unsigned long long *vbase_s = kbase_s + p.batch;
-  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + C::kStages), ring0 = smem_u32(smem);
-
+  const int hs = warp % U, rr = warp / U;      // head of the unit, token sub-row
+  WarpState &ws = reinterpret_cast<WarpState *>(smem + S::kWarp)[warp];
+  int *meta = reinterpret_cast<int *>(smem + S::kMeta);
+  const uint32_t full0 = smem_u32(smem + S::kBars), empty0 = full0 + 8 * C::kStages;
   const int g = p.h / p.kvh, slabs = p.kvh / U;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full0 + 8 * s, kCWarps);
-      mbar_init(empty0 + 8 * s, kCWarps);
+  {
+    int *prefix = meta + 4, *lens = prefix + p.batch + 1;
+    const bool cache_bases = p.batch <= kBaseCacheMaxBatch4;
+    unsigned long long *bases = reinterpret_cast<unsigned long long *>(meta + meta_ints4(p.batch));
+    if (threadIdx.x < 32)   // K row's part, K scales, V rows 2 c4 and 2 c4 + 1 (without the lane's 8 bytes)
+      reinterpret_cast<int4 *>(smem + S::kAt)[lane] =
+          make_int4(token_of_row<U>(lane >> 2) * UB + 16 * (lane & 3), token_of_row<U>(lane >> 2) * UB,
+                    token_of_row<U>(2 * (lane & 3)) * UB, token_of_row<U>(2 * (lane & 3) + 1) * UB);
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < C::kStages; ++s) {
+        mbar_init(full0 + 8 * s, kCWarps);
+        mbar_init(empty0 + 8 * s, kCWarps);
+      }
+      mbar_fence_init();
     }
-    mbar_fence_init();
-  }
-  for (int i = threadIdx.x; i < p.batch; i += kThreads4) {
-    int len = max(p.seq_lens[i], 0);
-    if constexpr (LOG) len = min(len, p.logit_rows);   // the logits have room for no more
-    lens[i] = len;
-    prefix[i + 1] = len > 0 ? ((len + TOK - 1) / TOK + kBoundaryCost) * slabs : 0;
-    if (cache_bases) {
-      const int64_t slot = p.slot_ids[i];
-      kbase_s[i] = p.k_table[slot];
-      vbase_s[i] = p.v_table[slot];
+    for (int i = threadIdx.x; i < p.batch; i += kThreads4) {
+      int len = max(p.seq_lens[i], 0);
+      if constexpr (LOG) len = min(len, p.logit_rows);   // the logits have room for no more
+      lens[i] = len;
+      prefix[i + 1] = len > 0 ? ((len + TOK - 1) / TOK + kBoundaryCost) * slabs : 0;
+      if (cache_bases) {
+        const int64_t slot = p.slot_ids[i];
+        bases[i] = p.k_table[slot];
+        bases[p.batch + i] = p.v_table[slot];
+      }
     }
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int carry = 0;
-    for (int base = 0; base < p.batch; base += 32) {
-      const int i = base + lane;
-      int v = i < p.batch ? prefix[i + 1] : 0;
+    __syncthreads();
+    if (warp == 0) {
+      int carry = 0;
+      for (int base = 0; base < p.batch; base += 32) {
+        const int i = base + lane;
+        int v = i < p.batch ? prefix[i + 1] : 0;
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int n = __shfl_up_sync(0xffffffffu, v, off);
-        if (lane >= off) v += n;
-      }
-      if (i < p.batch) prefix[i + 1] = carry + v;
-      carry += __shfl_sync(0xffffffffu, v, 31);
-    }
-    if (lane == 0) prefix[0] = 0;
-  }
-  __syncthreads();
-  pdl_launch_dependents();
-  const long long total = prefix[p.batch];
-  const int n_ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-  const bool active = static_cast<int>(blockIdx.x) < n_ctas;
-  const long long tau0 = active ? total * blockIdx.x / n_ctas : 0;
-  const long long tau1 = active ? total * (blockIdx.x + 1) / n_ctas : 0;
-  const int64_t row_bytes = static_cast<int64_t>(slabs) * UB;
-
-  // ---------------- copies ----------------
-  // Every warp fetches an eighth of the rows of the CTA's next tile into its ring stage, `n` tiles into the share, once
-  // all warps are done with what the stage held; false when a bounded wait ran out.  A single-unit cache is contiguous
-  // over tokens: one copy of K and one of V.  Otherwise a row of the unit (80 to 544 bytes) is one copy, a lane each.
-  const uint64_t policy = l2_policy_evict_first();
-  const auto fetch = [&](int n) -> bool {
-    if (cur.tile >= cur.tile_end) {
-      long long tau = cur.tau;
-      Piece pc{};
-      while (tau < tau1) {
-        pc = locate(prefix, p.batch, slabs, tau, tau1);
-        tau += pc.advance;
-        if (pc.tile_end > pc.tile_begin) break;
-      }
-      __syncwarp();
-      if (lane == 0) {
-        cur.tau = tau;
-        cur.tile = pc.tile_begin;
-        cur.tile_end = pc.tile_end;
-        if (pc.tile_end > pc.tile_begin) {
-          const int64_t slot = p.slot_ids[pc.b];
-          cur.k = reinterpret_cast<const char *>(cache_bases ? kbase_s[pc.b] : p.k_table[slot]) + pc.slab * UB;
-          cur.v = reinterpret_cast<const char *>(cache_bases ? vbase_s[pc.b] : p.v_table[slot]) + pc.slab * UB;
-          cur.seq_len = lens[pc.b];
+        for (int off = 1; off < 32; off <<= 1) {
+          const int n = __shfl_up_sync(0xffffffffu, v, off);
+          if (lane >= off) v += n;
         }
+        if (i < p.batch) prefix[i + 1] = carry + v;
+        carry += __shfl_sync(0xffffffffu, v, 31);
       }
-      __syncwarp();
-      if (cur.tile >= cur.tile_end) return true;   // the share is fetched
+      if (lane == 0) {
+        prefix[0] = 0;
+        const int n_ctas = min(static_cast<int>(gridDim.x), carry);
+        const bool active = static_cast<int>(blockIdx.x) < n_ctas;
+        meta[0] = carry;
+        meta[1] = n_ctas;
+        meta[2] = active ? static_cast<int>(static_cast<long long>(carry) * (blockIdx.x + 1) / n_ctas) : 0;
+      }
     }
-    constexpr int ROWS = TOK / kCWarps;
-    const int tile = cur.tile, s = n % C::kStages;
-    const int t0 = tile * TOK + warp * ROWS, nt = min(max(cur.seq_len - t0, 0), ROWS);
-    const int64_t src = t0 * row_bytes;
-    const char *kb = cur.k + src, *vb = cur.v + src;
-    if (n >= C::kStages && !mbar_wait(empty0 + 8 * s, ((n / C::kStages) - 1) & 1)) {
-      if (lane == 0) atomicExch(p.status, kKernelErrMagic);
-      return false;
-    }
-    const uint32_t dst = ring0 + s * C::kStage + warp * ROWS * UB;
-    __syncwarp();
+    __syncthreads();
     if (lane == 0) {
-      cur.tile = tile + 1;
-      mbar_arrive_expect_tx(full0 + 8 * s, 2u * nt * UB);
+      const int n_ctas = meta[1];
+      ws.tau = static_cast<int>(blockIdx.x) < n_ctas ? static_cast<int>(static_cast<long long>(meta[0]) * blockIdx.x / n_ctas) : 0;
+      ws.pieces = ws.copy_piece = 0;
     }
     __syncwarp();
-    if (slabs == 1) {
-      if (lane < 2 && nt > 0) bulk_g2s_hint(dst + lane * C::kTile, lane ? vb : kb, nt * UB, full0 + 8 * s, policy);
-    } else {
-      const int row = lane & 15;
-      static_assert(ROWS <= 16, "a lane per row of K and of V");
-      if (row < nt)
-        bulk_g2s_hint(dst + (lane >> 4) * C::kTile + row * UB, (lane >> 4 ? vb : kb) + row * row_bytes, UB, full0 + 8 * s, policy);
-    }
-    return true;
-  };
-  bool failed = false;
-  if (lane == 0) {
-    cur.tau = tau0;
-    cur.tile = cur.tile_end = 0;
+    look_ahead<UB>(p, ws, meta, slabs, 0, lane);
+    if (lane == 0) ws.copy_tile = ws.piece[0].tile_begin;
+    __syncwarp();
   }
-  __syncwarp();
-  for (int n = 0; n < C::kStages - 1; ++n) failed |= !fetch(n);
+  pdl_launch_dependents();
 
-  // ---------------- consumer warps ----------------
-  const int hs = warp % U, rr = warp / U;
-  const float sl2_base = p.scale * 1.4426950408889634f;
-  const int tid = threadIdx.x;
-  __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
+  bool failed = false;
+  for (int n = 0; n < C::kStages - 1; ++n) failed |= !fetch_tile<U>(p, smem, ws, n, slabs, warp, lane);
+
   if (blockIdx.x == 0) {   // sequences without context produce zeros; nobody owns a tile of theirs
+    const int *prefix = meta + 4;
     for (int b = 0; b < p.batch; ++b)
       if (prefix[b + 1] == prefix[b]) {
-        for (int i = tid; i < p.h * kHeadDim; i += kCWarps * 32) out[b * p.out_stride + i] = __float2bfloat16(0.f);
+        for (int i = threadIdx.x; i < p.h * kHeadDim; i += kThreads4)
+          static_cast<__nv_bfloat16 *>(p.out)[b * p.out_stride + i] = __float2bfloat16(0.f);
         if (p.lse)
-          for (int i = tid; i < p.h; i += kCWarps * 32) p.lse[b * p.h + i] = -INFINITY;
+          for (int i = threadIdx.x; i < p.h; i += kThreads4) p.lse[b * p.h + i] = -INFINITY;
       }
   }
   int it = 0;
-  bool first_piece = true;
-  for (long long tau = tau0; tau < tau1;) {
-    const Piece pc = locate(prefix, p.batch, slabs, tau, tau1);
-    if (pc.tile_end <= pc.tile_begin) {
-      tau += pc.advance;
-      continue;
-    }
-    const int seq_len = lens[pc.b];
-    const int kv_head = pc.slab * U + hs;
-    const int64_t append_off = p.new_key ? p.byte_off[pc.b] : -1;
+  for (int now = 0; now < ws.pieces; ++now) {
+    if (now > 0) look_ahead<UB>(p, ws, meta, slabs, now, lane);
+    const PieceRec &pc = ws.piece[now % kPieces];
     if (p.overlap == 2) pdl_wait_prior_grid();
-    WarpAttn4<NB> st;
-    st.start(static_cast<const __nv_bfloat16 *>(p.q) + pc.b * p.q_stride + kv_head * g * kHeadDim, g,
-             sl2_base * p.k_scale[kv_head], lane);
-    float *lg = nullptr;
-    if constexpr (LOG) lg = p.logits + (static_cast<size_t>(pc.b) * p.kvh + kv_head) * p.logit_rows * g;
-    for (int tile = pc.tile_begin; tile < pc.tile_end; ++tile, ++it) {
-      const int s = it % C::kStages;
-      // the stage of the tile before this one, which the other warps are likely done with
-      if (!failed && !fetch(it + C::kStages - 1)) failed = true;
-      if (!failed && !mbar_wait(full0 + 8 * s, (it / C::kStages) & 1)) failed = true;
-      if (failed) continue;
-      unsigned char *kt = smem + s * C::kStage + hs * 64, *vt = kt + C::kTile;
-      const int sc = U * 64 + hs * 4 - hs * 64;
-      const int t0 = tile * TOK;
-      const int fresh = seq_len - 1 - t0;   // position of the newest token in the tile
-      bool wrote = false;
-      if (append_off >= 0 && fresh < TOK && (fresh / 16) % R == rr) {
-        // Fused step: this warp owns the newest token's row of its kv head.  The copy brought whatever the range
-        // held; quantise the step's row over it, in the stage and in the range.
-        char *kd, *vd;
-        if (cache_bases) {
-          kd = reinterpret_cast<char *>(kbase_s[pc.b]);
-          vd = reinterpret_cast<char *>(vbase_s[pc.b]);
-        } else {
-          const int64_t slot = p.slot_ids[pc.b];
-          kd = reinterpret_cast<char *>(p.k_table[slot]);
-          vd = reinterpret_cast<char *>(p.v_table[slot]);
-        }
-        const int64_t dst = append_off + pc.slab * UB + hs * 64;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(kv ? p.new_value : p.new_key) +
-                                     pc.b * (kv ? p.new_value_stride : p.new_key_stride) + kv_head * kHeadDim + lane * 4;
-          const uint2 w = __ldg(reinterpret_cast<const uint2 *>(src));
-          const float x[4] = {bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
-          uint32_t bits, s8;
-          quantise4(x, (kv ? p.v_scale : p.k_scale)[kv_head], &bits, &s8);
-          unsigned char *row = (kv ? vt : kt) + fresh * UB;
-          char *far = (kv ? vd : kd) + dst;
-          const int at = 8 * (lane & 7) + 2 * (lane >> 3);
-          *reinterpret_cast<uint16_t *>(row + at) = static_cast<uint16_t>(bits);
-          *reinterpret_cast<uint16_t *>(far + at) = static_cast<uint16_t>(bits);
-          if ((lane & 7) == 0) {
-            row[sc + (lane >> 3)] = static_cast<unsigned char>(s8);
-            far[sc + (lane >> 3)] = static_cast<char>(s8);
-          }
-        }
-        __syncwarp();
-        wrote = true;
-      }
-      const int n_tok = seq_len - t0 - 16 * rr;
-      if (n_tok > 0)
-        st.template tile<U, LOG>(kt + 16 * rr * UB, vt + 16 * rr * UB, sc, n_tok, lane,
-                                 LOG ? lg + static_cast<size_t>(t0 + 16 * rr) * g : nullptr, g);
-      if (wrote) fence_proxy_async();   // before the copy engine refills the stage
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty0 + 8 * s);
+    const int64_t append_off = p.new_key ? p.byte_off[pc.b] : -1;
+    const bool fresh = append_off >= 0 && pc.tile_end == pc.tiles && ((pc.seq_len - 1) % TOK / 16) % R == rr;
+    if (fresh) append_row<U>(p, ws, pc, hs, append_off, lane);   // this warp owns the newest token's row of its head
+    const int got = run_piece<U, NB, LOG>(p, now, it, failed, fresh);
+    failed = got & 1;
+    it += pc.tile_end - pc.tile_begin;
+    if (got & 2) {
+      const long long total = meta[0];
+      const int n_ctas = meta[1];
+      merge_head<U, R, HEADS>(p, pc.b, pc.slab * U + hs, pc.stream_begin, total, n_ctas, owner_of(pc.stream_begin + kBoundaryCost, total, n_ctas),
+                              owner_of(pc.stream_end - 1, total, n_ctas), lane, g);
     }
-    st.finish(lane);
-
-    const bool whole = pc.tile_begin == 0 && pc.tile_end == pc.tiles_in_stream;
-    if (R == 1 && whole) {
-      const int r4 = lane >> 2, c4 = lane & 3;
-      const float vs = p.v_scale[kv_head];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int head = nb * 8 + 2 * c4 + e;
-          if (head < g) {
-            const float inv = vs / st.lrun[nb][e];
-            const int hq = kv_head * g + head;
-            __nv_bfloat16 *dst = out + pc.b * p.out_stride + hq * kHeadDim;
-#pragma unroll
-            for (int mb = 0; mb < 8; ++mb)   // dims d, d + 1 are the two fragment rows
-              *reinterpret_cast<uint32_t *>(dst + WarpAttn4<NB>::dim_of(mb, 0, r4)) =
-                  pack_bf16(st.o[nb][mb][e] * inv, st.o[nb][mb][2 + e] * inv);
-            if (r4 == 0) write_stats(p, pc.b * p.h + hq, st.mrun[nb][e], st.lrun[nb][e]);
-          }
-        }
-      }
-    } else {
-      if (p.overlap) pdl_wait_prior_grid();
-      float *slot_base = p.fl_part + (static_cast<size_t>(blockIdx.x) * 2 + (first_piece ? 0 : 1)) * kCWarps * HEADS * kPartRow;
-      st.template store<kPartRow>(slot_base + warp * HEADS * kPartRow, lane, g);
-      __threadfence();
-      named_bar_sync(1, kCWarps * 32);
-      const int c_first = owner_of(pc.stream_begin + kBoundaryCost, total, n_ctas);
-      const int c_last = owner_of(pc.stream_end - 1, total, n_ctas);
-      if (tid == 0) {
-        unsigned *ctr = p.fl_count + pc.b * slabs + pc.slab;
-        const unsigned old = atomicAdd(ctr, 1u);
-        const int last = old + 1 == static_cast<unsigned>(c_last - c_first + 1);
-        if (last) *ctr = 0u;
-        flags[0] = last;
-      }
-      named_bar_sync(1, kCWarps * 32);
-      const bool merger = flags[0] != 0;
-      named_bar_sync(1, kCWarps * 32);
-      if (merger) {
-        merge_stream<kCWarps, U, R, HEADS, true, false>(p, pc, total, n_ctas, c_first, c_last, warp, lane, g);
-        if (R > 1) named_bar_sync(1, kCWarps * 32);   // this CTA's next piece may publish to the slot just read
-      }
-    }
-    first_piece = false;
-    tau += pc.advance;
+    // a stream that lies wholly in this CTA's share used slot 1, as the next piece may
+    if (R > 1 && pc.tile_begin == 0 && pc.tile_end == pc.tiles) named_bar_sync(1, kCWarps * 32);
   }
-  if (failed && lane == 0) atomicExch(p.status, kKernelErrMagic);
 }
 
 template <int U, int NB, bool LOG>
 int launch4(const AttnParams &p_in, cudaStream_t stream) {
   AttnParams p = p_in;
   p.n_ctas = (NB == 1 ? 2 : 1) * kFlatSms;
-  const int smem = smem_bytes4<U>(p.batch);
+  const int smem = Layout4<U, NB>::bytes(p.batch);
   static SmemOptIn opt_in;
   if (!opt_in.ensure(attn_int4_kernel<U, NB, LOG>, smem)) return VT_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};

@@ -547,18 +547,42 @@ __device__ __noinline__ void append_row(const AttnParams &p, WarpState &ws, cons
   __syncwarp();
 }
 
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {   // does not suspend
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Every warp fetches an eighth of the rows of the CTA's next tile into its ring stage, `n` tiles into the share, once all
-// warps are done with what the stage held; false when a bounded wait ran out.  A single-unit cache is contiguous over
+// warps are done with what the stage held.  1: fetched (or the share is), 0: the stage is still in use and `wait` is
+// false, -1: a bounded wait ran out.  A single-unit cache is contiguous over
 // tokens: one copy of K and one of V.  Otherwise a row of the unit (80 to 544 bytes) is one copy, a lane each.
 template <int U>
-__device__ __forceinline__ bool fetch_tile(const AttnParams &p, unsigned char *smem, WarpState &ws, int n, int slabs, int warp, int lane) {
+__device__ __forceinline__ int fetch_tile(const AttnParams &p, unsigned char *smem, WarpState &ws, int n, int slabs, int warp, int lane,
+                                          bool wait) {
   using C = Cfg4<U>;
   constexpr int UB = C::UB, ROWS = C::TOK / kCWarps;
   static_assert(ROWS <= 16, "a lane per row of K and of V");
   int piece = ws.copy_piece, tile = ws.copy_tile;
-  if (piece >= ws.pieces) return true;   // the share is fetched
-  const PieceRec &pc = ws.piece[piece % kPieces];
+  if (piece >= ws.pieces) return 1;
   const int s = n % C::kStages;
+  const uint32_t bar = smem_u32(smem) + C::kStages * C::kStage + 8 * s;   // full; the empty ones follow
+  if (n >= C::kStages) {
+    const uint32_t empty = bar + 8 * C::kStages, parity = ((n / C::kStages) - 1) & 1;
+    if (!wait) {
+      if (!__all_sync(0xffffffffu, mbar_test(empty, parity))) return 0;
+    } else if (!mbar_wait(empty, parity)) {
+      if (lane == 0) atomicExch(p.status, kKernelErrMagic);
+      return -1;
+    }
+  }
+  const PieceRec &pc = ws.piece[piece % kPieces];
   const int t0 = tile * C::TOK + warp * ROWS, nt = min(max(pc.seq_len - t0, 0), ROWS);
   const int64_t src = static_cast<int64_t>(t0) * (slabs * UB);
   const char *kb = pc.k + src, *vb = pc.v + src;
@@ -566,11 +590,6 @@ __device__ __forceinline__ bool fetch_tile(const AttnParams &p, unsigned char *s
   if (tile >= pc.tile_end) {
     ++piece;
     tile = ws.piece[piece % kPieces].tile_begin;
-  }
-  const uint32_t bar = smem_u32(smem) + C::kStages * C::kStage + 8 * s;   // full; the empty ones follow
-  if (n >= C::kStages && !mbar_wait(bar + 8 * C::kStages, ((n / C::kStages) - 1) & 1)) {
-    if (lane == 0) atomicExch(p.status, kKernelErrMagic);
-    return false;
   }
   const uint32_t dst = smem_u32(smem) + s * C::kStage + warp * ROWS * UB;
   __syncwarp();
@@ -589,7 +608,7 @@ __device__ __forceinline__ bool fetch_tile(const AttnParams &p, unsigned char *s
       bulk_g2s_hint(dst + (lane >> 4) * C::kTile + row * UB, (lane >> 4 ? vb : kb) + static_cast<int64_t>(row) * (slabs * UB), UB, bar,
                     policy);
   }
-  return true;
+  return 1;
 }
 
 // Piece `now` of the CTA's share, the `it`-th tile on: attention, then either the result or a published state and a
@@ -618,8 +637,8 @@ __device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, bool
   int left = pc.seq_len - pc.tile_begin * TOK;   // tokens from the tile's first to the end of the context
   for (int tiles = pc.tile_end - pc.tile_begin; tiles > 0; --tiles, ++it, left -= TOK) {
     const int s = it % C::kStages;
-    // the stage of the tile before this one, which the other warps are likely done with
-    if (!failed && !fetch_tile<U>(p, smem, ws, it + C::kStages - 1, slabs, warp, lane)) failed = true;
+    // into the stage of the tile before this one: now if the other warps are done with it, else after this tile
+    const int fetched = failed ? 1 : fetch_tile<U>(p, smem, ws, it + C::kStages - 1, slabs, warp, lane, false);
     if (!failed && !mbar_wait(full0 + 8 * s, (it / C::kStages) & 1)) failed = true;
     if (failed) continue;
     unsigned char *kt = smem + s * C::kStage + hs * 64;
@@ -647,6 +666,7 @@ __device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, bool
     if (overlay) fence_proxy_async();   // before the copy engine refills the stage
     __syncwarp();
     if (lane == 0) mbar_arrive(empty0 + 8 * s);
+    if (fetched == 0 && fetch_tile<U>(p, smem, ws, it + C::kStages - 1, slabs, warp, lane, true) < 0) failed = true;
   }
   st.finish(lane);
 
@@ -769,7 +789,7 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(c
   pdl_launch_dependents();
 
   bool failed = false;
-  for (int n = 0; n < C::kStages - 1; ++n) failed |= !fetch_tile<U>(p, smem, ws, n, slabs, warp, lane);
+  for (int n = 0; n < C::kStages - 1; ++n) failed |= fetch_tile<U>(p, smem, ws, n, slabs, warp, lane, true) < 0;
 
   if (blockIdx.x == 0) {   // sequences without context produce zeros; nobody owns a tile of theirs
     const int *prefix = meta + 4;

@@ -30,6 +30,7 @@
 #include "vt_mma.cuh"
 #include "vt_mma_f8.cuh"
 #include "vt_attn_flat_sched.cuh"
+#include "vt_umma.cuh"
 
 namespace vt {
 namespace {
@@ -37,7 +38,6 @@ namespace {
 constexpr int kCWarps = 8;                 // consumer warps = heads of a unit x token sub-rows of a tile
 constexpr int kThreads4 = kCWarps * 32;
 constexpr int kRingBudget = 106000;        // two CTAs per SM with their tables
-constexpr int kBaseCacheMaxBatch4 = 256;
 constexpr float kPScaleLog2 = 6.f;         // P is carried times 2^6
 
 template <int U>
@@ -87,10 +87,10 @@ struct WarpAttn4 {
     return 32 * (mb >> 1) + 4 * r4 + 2 * (mb & 1) + half;
   }
 
-  // Per q head of the warp, in shared memory (ten registers the tile loop would spill): -8 sum q of every group, and the
-  // factor from partial logits to the log2 domain.
-  static constexpr int kQRow = 6;   // floats: 4 offsets, factor, pad
-  static constexpr int kQFloats = NB * 8 * kQRow;
+  // Per pair of q heads of the warp, in shared memory (ten registers the tile loop would spill): -8 sum q of every group,
+  // and the factor from partial logits to the log2 domain.
+  static constexpr int kQRow = 6;   // pairs of floats: 4 offsets, factor, pad
+  static constexpr int kQFloats = NB * 4 * kQRow * 2;
 
   __device__ __forceinline__ void start(const __nv_bfloat16 *qrow, int g, float sl2, int lane, float *qs) {
     const int r4 = lane >> 2, c4 = lane & 3;
@@ -131,10 +131,10 @@ struct WarpAttn4 {
         sum[G] += __shfl_xor_sync(0xffffffffu, sum[G], 2);
       }
       if (c4 == 0) {
-        float *mine = qs + head * kQRow;
+        float *mine = qs + (head >> 1) * kQRow * 2 + (head & 1);
 #pragma unroll
-        for (int G = 0; G < 4; ++G) mine[G] = sum[G] * -4.76837158203125e-7f;   // -8 2^-24
-        mine[4] = sl2 * (16777216.f / f);   // 2^24 of the nibbles, 1 / f of Q
+        for (int G = 0; G < 4; ++G) mine[2 * G] = sum[G] * -4.76837158203125e-7f;   // -8 2^-24
+        mine[8] = sl2 * (16777216.f / f);   // 2^24 of the nibbles, 1 / f of Q
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -176,24 +176,26 @@ struct WarpAttn4 {
     }
     const uint32_t a01 = e4m3x2_to_f16x2(wsa), a23 = e4m3x2_to_f16x2(wsa >> 16);
     const uint32_t b01 = e4m3x2_to_f16x2(wsb), b23 = e4m3x2_to_f16x2(wsb >> 16);
-    const float ga[4] = {f16_lo(a01), f16_hi(a01), f16_lo(a23), f16_hi(a23)};
-    const float gb[4] = {f16_lo(b01), f16_hi(b01), f16_lo(b23), f16_hi(b23)};
+    // pairs (scale, scale) for the two heads of a column pair
+    const uint64_t ga[4] = {f2_pack(f16_lo(a01), f16_lo(a01)), f2_pack(f16_hi(a01), f16_hi(a01)), f2_pack(f16_lo(a23), f16_lo(a23)),
+                            f2_pack(f16_hi(a23), f16_hi(a23))};
+    const uint64_t gb[4] = {f2_pack(f16_lo(b01), f16_lo(b01)), f2_pack(f16_hi(b01), f16_hi(b01)), f2_pack(f16_lo(b23), f16_lo(b23)),
+                            f2_pack(f16_hi(b23), f16_hi(b23))};
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      // the "- 8" of a group is added to its sum here, on the FMA pipe: as the start value of the accumulators it
-      // costs a move per register on the ALU pipe, which is the busy one
-      const float *q0 = qs + (nb * 8 + 2 * c4) * kQRow, *q1 = q0 + kQRow;
+      // The "- 8" of a group is added to its sum here, on the FMA pipe (two lanes an instruction): as the start value of
+      // the accumulators it costs a move per register on the ALU pipe, which is the busy one.
+      const uint64_t *qp = reinterpret_cast<const uint64_t *>(qs) + (nb * 4 + c4) * kQRow;
+      uint64_t sa = 0, sb = 0;
 #pragma unroll
       for (int G = 0; G < 4; ++G) {
-        const float x0 = acc[nb][G][0] + q0[G], x1 = acc[nb][G][1] + q1[G];
-        const float x2 = acc[nb][G][2] + q0[G], x3 = acc[nb][G][3] + q1[G];
-        s[nb][0] = G ? fmaf(ga[G], x0, s[nb][0]) : ga[G] * x0;
-        s[nb][1] = G ? fmaf(ga[G], x1, s[nb][1]) : ga[G] * x1;
-        s[nb][2] = G ? fmaf(gb[G], x2, s[nb][2]) : gb[G] * x2;
-        s[nb][3] = G ? fmaf(gb[G], x3, s[nb][3]) : gb[G] * x3;
+        const uint64_t off = qp[G];
+        const uint64_t xa = f2_add(f2_pack(acc[nb][G][0], acc[nb][G][1]), off), xb = f2_add(f2_pack(acc[nb][G][2], acc[nb][G][3]), off);
+        sa = G ? f2_fma(ga[G], xa, sa) : f2_mul(ga[G], xa);
+        sb = G ? f2_fma(gb[G], xb, sb) : f2_mul(gb[G], xb);
       }
-      s[nb][0] *= q0[4]; s[nb][1] *= q1[4];
-      s[nb][2] *= q0[4]; s[nb][3] *= q1[4];
+      f2_unpack(f2_mul(sa, qp[4]), s[nb][0], s[nb][1]);
+      f2_unpack(f2_mul(sb, qp[4]), s[nb][2], s[nb][3]);
     }
   }
 
@@ -384,33 +386,28 @@ struct WarpAttn4 {
   }
 };
 
-// What a warp keeps in shared memory, because registers held over the tile loop are the scarce resource (spills go to
-// an L1 that the rings leave 20 KB of: a handful of reloads per tile cost 200 of 440 us): the pieces of its share ahead
-// of it and where its copies stand.
+// What is needed once per piece is kept in shared memory, because registers held over the tile loop are the scarce
+// resource (spills go to an L1 that the rings leave 20 KB of: a handful of reloads per tile cost 200 of 440 us).
 struct PieceRec {
   const char *k, *v;               // the unit's rows of the piece's sequence
   int b, slab, tile_begin, tile_end, tiles, seq_len;   // as Piece; tiles = of the whole stream
   int stream_begin, stream_end;
 };
-constexpr int kPieces = 4;         // the copies run at most two tiles ahead, so they stay within the next three pieces
-struct alignas(16) WarpState {
-  PieceRec piece[kPieces];
-  int tau, pieces;                 // position after, and number of, the pieces looked up so far
-  int copy_piece, copy_tile;       // next tile to fetch
-  uint32_t fresh[2][32];           // fused step: the lanes' 16 bits and scale byte (<< 16) of the newest K and V row
-};
+constexpr int kPieces = 32;        // pieces looked up at a time; a share of more (many one-tile sequences) goes in rounds
+struct FreshRow { uint32_t w[2][32]; };   // fused step: a warp's lanes' 16 bits and scale byte (<< 16) of the newest K and V row
 
-// ring | barriers | warp states | q statistics | flags | prefix[batch + 1] | lens[batch] | (pad to 8) | kbase[batch] | vbase[batch]
+// ring | barriers | pieces | fresh rows | q statistics | fragment offsets | flags | prefix[batch + 1] | lens[batch]
 __host__ __device__ constexpr int meta_ints4(int batch) { return ((2 * batch + 1 + 4) + 1) / 2 * 2; }
 template <int U, int NB>
 struct Layout4 {
   static constexpr int kBars = Cfg4<U>::kStages * Cfg4<U>::kStage;
-  static constexpr int kWarp = kBars + Cfg4<U>::kStages * 16;
-  static constexpr int kQ = kWarp + kCWarps * static_cast<int>(sizeof(WarpState));
+  static constexpr int kPiece = kBars + Cfg4<U>::kStages * 16;
+  static constexpr int kFresh = kPiece + kPieces * static_cast<int>(sizeof(PieceRec));
+  static constexpr int kQ = kFresh + kCWarps * static_cast<int>(sizeof(FreshRow));
   static constexpr int kAt = kQ + kCWarps * WarpAttn4<NB>::kQFloats * 4;      // per lane: fragment offsets in a tile
-  static constexpr int kMeta = kAt + 32 * 16;   // 4 ints: total positions, CTAs, end of the share
-  static constexpr int bytes(int batch) { return kMeta + meta_ints4(batch) * 4 + (batch <= kBaseCacheMaxBatch4 ? batch * 16 : 0); }
-  static_assert(sizeof(WarpState) % 8 == 0 && kQ % 8 == 0 && kAt % 16 == 0 && kMeta % 8 == 0, "alignment");
+  static constexpr int kMeta = kAt + 32 * 16;                                 // 4 ints: total positions, CTAs, pieces of the share
+  static constexpr int bytes(int batch) { return kMeta + meta_ints4(batch) * 4; }
+  static_assert(kPiece % 8 == 0 && kQ % 16 == 0 && kAt % 16 == 0 && kMeta % 8 == 0, "alignment");
 };
 
 // Merge of one kv head of a stream by the warp that drew its last ticket (scratch layout of merge_stream, but a ticket
@@ -500,37 +497,36 @@ __device__ __noinline__ void merge_head(const AttnParams &p, int b, int kv_head,
   }
 }
 
-// Looks up pieces of the share until kPieces - 1 lie ahead of piece `now`, or the share ends.  meta: the CTA's flags.
+// Looks up the next pieces of positions [meta[3], end), one warp for the CTA: meta[2] = how many that hold tiles, meta[3]
+// = position behind them.
 template <int UB>
-__device__ __noinline__ void look_ahead(const AttnParams &p, WarpState &ws, const int *meta, int slabs, int now, int lane) {
+__device__ __noinline__ void look_up(const AttnParams &p, PieceRec *rec, int *meta, int slabs, int end, int lane) {
   const int *prefix = meta + 4, *lens = prefix + p.batch + 1;
-  const unsigned long long *bases = reinterpret_cast<const unsigned long long *>(meta + meta_ints4(p.batch));
-  int tau = ws.tau, n = ws.pieces;
-  const int end = meta[2];
-  __syncwarp();
-  while (tau < end && n < now + kPieces) {
+  int n = 0, tau = meta[3];
+  while (tau < end && n < kPieces) {
     const Piece pc = locate(prefix, p.batch, slabs, tau, end);
     tau += pc.advance;
     if (pc.tile_end <= pc.tile_begin) continue;   // only phantom positions of this stream fall into the share
     if (lane == 0) {
-      PieceRec &r = ws.piece[n % kPieces];
-      const bool cached = p.batch <= kBaseCacheMaxBatch4;
-      const int64_t slot = cached ? 0 : p.slot_ids[pc.b];
-      r.k = reinterpret_cast<const char *>(cached ? bases[pc.b] : p.k_table[slot]) + pc.slab * UB;
-      r.v = reinterpret_cast<const char *>(cached ? bases[p.batch + pc.b] : p.v_table[slot]) + pc.slab * UB;
+      PieceRec &r = rec[n];
       r.b = pc.b; r.slab = pc.slab; r.tile_begin = pc.tile_begin; r.tile_end = pc.tile_end; r.tiles = pc.tiles_in_stream;
       r.seq_len = lens[pc.b];
       r.stream_begin = static_cast<int>(pc.stream_begin); r.stream_end = static_cast<int>(pc.stream_end);
     }
     ++n;
   }
-  if (lane == 0) { ws.tau = tau; ws.pieces = n; }
   __syncwarp();
+  for (int i = lane; i < n; i += 32) {   // the ranges' addresses, all pieces at once
+    const int64_t slot = p.slot_ids[rec[i].b];
+    rec[i].k = reinterpret_cast<const char *>(p.k_table[slot]) + rec[i].slab * UB;
+    rec[i].v = reinterpret_cast<const char *>(p.v_table[slot]) + rec[i].slab * UB;
+  }
+  if (lane == 0) { meta[2] = n; meta[3] = tau; }
 }
 
 // Fused step: quantises the step's row of this warp's head, stores it into the ranges and leaves the lanes' bits in ws.
 template <int U>
-__device__ __noinline__ void append_row(const AttnParams &p, WarpState &ws, const PieceRec &pc, int hs, int64_t off, int lane) {
+__device__ __noinline__ void append_row(const AttnParams &p, FreshRow &out, const PieceRec &pc, int hs, int64_t off, int lane) {
   const int kv_head = pc.slab * U + hs, at = 8 * (lane & 7) + 2 * (lane >> 3);
   for (int kv = 0; kv < 2; ++kv) {
     const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(kv ? p.new_value : p.new_key) +
@@ -542,7 +538,7 @@ __device__ __noinline__ void append_row(const AttnParams &p, WarpState &ws, cons
     char *far = const_cast<char *>(kv ? pc.v : pc.k) + off;   // the unit's bytes of the row
     *reinterpret_cast<uint16_t *>(far + hs * 64 + at) = static_cast<uint16_t>(bits);
     if ((lane & 7) == 0) far[U * 64 + hs * 4 + (lane >> 3)] = static_cast<char>(s8);
-    ws.fresh[kv][lane] = bits | s8 << 16;
+    out.w[kv][lane] = bits | s8 << 16;
   }
   __syncwarp();
 }
@@ -559,75 +555,74 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {   // 
   return ok != 0;
 }
 
-// Every warp fetches an eighth of the rows of the CTA's next tile into its ring stage, `n` tiles into the share, once all
-// warps are done with what the stage held.  1: fetched (or the share is), 0: the stage is still in use and `wait` is
-// false, -1: a bounded wait ran out.  A single-unit cache is contiguous over
-// tokens: one copy of K and one of V.  Otherwise a row of the unit (80 to 544 bytes) is one copy, a lane each.
+// Fetches tile `tile` of a piece into ring stage s; the whole warp calls it.  `use` = how often the stage was filled
+// before.  1: done, 0: the stage is still in use and `wait` is false, -1: a bounded wait ran out.  A single-unit cache is
+// contiguous over tokens: one copy of K and one of V.  Otherwise a row of the unit (80 to 544 bytes) is one copy.
 template <int U>
-__device__ __forceinline__ int fetch_tile(const AttnParams &p, unsigned char *smem, WarpState &ws, int n, int slabs, int warp, int lane,
-                                          bool wait) {
+__device__ __forceinline__ int fetch_tile(const AttnParams &p, unsigned char *smem, const PieceRec &pc, int tile, int s, int use,
+                                          int slabs, int lane, bool wait) {
   using C = Cfg4<U>;
-  constexpr int UB = C::UB, ROWS = C::TOK / kCWarps;
-  static_assert(ROWS <= 16, "a lane per row of K and of V");
-  int piece = ws.copy_piece, tile = ws.copy_tile;
-  if (piece >= ws.pieces) return 1;
-  const int s = n % C::kStages;
+  constexpr int UB = C::UB;
   const uint32_t bar = smem_u32(smem) + C::kStages * C::kStage + 8 * s;   // full; the empty ones follow
-  if (n >= C::kStages) {
-    const uint32_t empty = bar + 8 * C::kStages, parity = ((n / C::kStages) - 1) & 1;
+  if (use > 0) {
+    const uint32_t empty = bar + 8 * C::kStages, parity = (use - 1) & 1;
     if (!wait) {
       if (!__all_sync(0xffffffffu, mbar_test(empty, parity))) return 0;
-    } else if (!mbar_wait(empty, parity)) {
+    } else if (!__all_sync(0xffffffffu, mbar_wait(empty, parity))) {
       if (lane == 0) atomicExch(p.status, kKernelErrMagic);
       return -1;
     }
   }
-  const PieceRec &pc = ws.piece[piece % kPieces];
-  const int t0 = tile * C::TOK + warp * ROWS, nt = min(max(pc.seq_len - t0, 0), ROWS);
+  const int t0 = tile * C::TOK, nt = min(pc.seq_len - t0, C::TOK);
   const int64_t src = static_cast<int64_t>(t0) * (slabs * UB);
   const char *kb = pc.k + src, *vb = pc.v + src;
-  ++tile;
-  if (tile >= pc.tile_end) {
-    ++piece;
-    tile = ws.piece[piece % kPieces].tile_begin;
-  }
-  const uint32_t dst = smem_u32(smem) + s * C::kStage + warp * ROWS * UB;
-  __syncwarp();
-  if (lane == 0) {
-    ws.copy_piece = piece;
-    ws.copy_tile = tile;
-    mbar_arrive_expect_tx(bar, 2u * nt * UB);
-  }
-  __syncwarp();
+  const uint32_t dst = smem_u32(smem) + s * C::kStage;
   const uint64_t policy = l2_policy_evict_first();
+  if (lane == 0) mbar_arrive_expect_tx(bar, 2u * nt * UB);
+  __syncwarp();
   if (slabs == 1) {
-    if (lane < 2 && nt > 0) bulk_g2s_hint(dst + lane * C::kTile, lane ? vb : kb, nt * UB, bar, policy);
+    if (lane == 0) {
+      bulk_g2s_hint(dst, kb, nt * UB, bar, policy);
+      bulk_g2s_hint(dst + C::kTile, vb, nt * UB, bar, policy);
+    }
   } else {
-    const int row = lane & 15;
-    if (row < nt)
-      bulk_g2s_hint(dst + (lane >> 4) * C::kTile + row * UB, (lane >> 4 ? vb : kb) + static_cast<int64_t>(row) * (slabs * UB), UB, bar,
-                    policy);
+    for (int row = lane; row < nt; row += 32) {
+      bulk_g2s_hint(dst + row * UB, kb + static_cast<int64_t>(row) * (slabs * UB), UB, bar, policy);
+      bulk_g2s_hint(dst + C::kTile + row * UB, vb + static_cast<int64_t>(row) * (slabs * UB), UB, bar, policy);
+    }
   }
   return 1;
+}
+
+// Moves a copy position `n` tiles on in the list of pieces.
+__device__ __forceinline__ void next_copy(const PieceRec *rec, int pieces, int &piece, int &tile, int n) {
+  tile += n;
+  while (piece < pieces && tile >= rec[piece].tile_end) {
+    const int over = tile - rec[piece].tile_end;
+    ++piece;
+    if (piece < pieces) tile = rec[piece].tile_begin + over;
+  }
 }
 
 // Piece `now` of the CTA's share, the `it`-th tile on: attention, then either the result or a published state and a
 // ticket.  Bit 0: a bounded wait ran out; bit 1: this warp drew the last ticket of its head.  A function of its own, with
 // no calls inside: what the compiler would otherwise keep on the stack across the merge it reloads in the tile loop.
 template <int U, int NB, bool LOG>
-__device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, bool failed, bool fresh) {
+__device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, int state, int &copy_piece, int &copy_tile) {
   using C = Cfg4<U>;
   using S = Layout4<U, NB>;
   constexpr int R = C::R, UB = C::UB, TOK = C::TOK, HEADS = NB * 8;
   extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hs = warp % U, rr = warp / U;      // head of the unit, token sub-row
-  WarpState &ws = reinterpret_cast<WarpState *>(smem + S::kWarp)[warp];
   float *qs = reinterpret_cast<float *>(smem + S::kQ) + warp * WarpAttn4<NB>::kQFloats;
   const int *meta = reinterpret_cast<const int *>(smem + S::kMeta);
   const uint32_t full0 = smem_u32(smem + S::kBars), empty0 = full0 + 8 * C::kStages;
   const int g = p.h / p.kvh, slabs = p.kvh / U;
-  const PieceRec &pc = ws.piece[now % kPieces];
+  const PieceRec *rec = reinterpret_cast<const PieceRec *>(smem + S::kPiece);
+  const PieceRec &pc = rec[now];
+  bool failed = state & 1;
+  const bool fresh = state & 2;   // this warp overlays the newest token's row; bit 2: the CTA's first piece
   WarpAttn4<NB> st;
   {
     const int kv_head = pc.slab * U + hs;
@@ -637,8 +632,12 @@ __device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, bool
   int left = pc.seq_len - pc.tile_begin * TOK;   // tokens from the tile's first to the end of the context
   for (int tiles = pc.tile_end - pc.tile_begin; tiles > 0; --tiles, ++it, left -= TOK) {
     const int s = it % C::kStages;
-    // into the stage of the tile before this one: now if the other warps are done with it, else after this tile
-    const int fetched = failed ? 1 : fetch_tile<U>(p, smem, ws, it + C::kStages - 1, slabs, warp, lane, false);
+    // Warp n % 8 fetches tile n, into the stage of the tile before this one: now if all warps are done with that, else
+    // after this tile.
+    const int n = it + C::kStages - 1;
+    const bool mine = (n & (kCWarps - 1)) == warp && copy_piece < meta[2];
+    int fetched = 1;
+    if (mine && !failed) fetched = fetch_tile<U>(p, smem, rec[copy_piece], copy_tile, n % C::kStages, n / C::kStages, slabs, lane, false);
     if (!failed && !mbar_wait(full0 + 8 * s, (it / C::kStages) & 1)) failed = true;
     if (failed) continue;
     unsigned char *kt = smem + s * C::kStage + hs * 64;
@@ -648,7 +647,7 @@ __device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, bool
       const int at = 8 * (lane & 7) + 2 * (lane >> 3);
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        const uint32_t w = ws.fresh[kv][lane];
+        const uint32_t w = reinterpret_cast<const FreshRow *>(smem + S::kFresh)[warp].w[kv][lane];
         unsigned char *row = kt + kv * C::kTile + (left - 1) * UB;
         *reinterpret_cast<uint16_t *>(row + at) = static_cast<uint16_t>(w);
         if ((lane & 7) == 0) row[kSc - hs * 60 + (lane >> 3)] = static_cast<unsigned char>(w >> 16);
@@ -666,7 +665,9 @@ __device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, bool
     if (overlay) fence_proxy_async();   // before the copy engine refills the stage
     __syncwarp();
     if (lane == 0) mbar_arrive(empty0 + 8 * s);
-    if (fetched == 0 && fetch_tile<U>(p, smem, ws, it + C::kStages - 1, slabs, warp, lane, true) < 0) failed = true;
+    if (fetched == 0 && fetch_tile<U>(p, smem, rec[copy_piece], copy_tile, n % C::kStages, n / C::kStages, slabs, lane, true) < 0)
+      failed = true;
+    if (mine) next_copy(rec, meta[2], copy_piece, copy_tile, kCWarps);
   }
   st.finish(lane);
 
@@ -694,7 +695,7 @@ __device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, bool
     }
   } else {
     if (p.overlap) pdl_wait_prior_grid();   // the scratch is shared with the previous launch
-    float *slot_base = p.fl_part + (static_cast<size_t>(blockIdx.x) * 2 + (now == 0 ? 0 : 1)) * kCWarps * HEADS * kPartRow;
+    float *slot_base = p.fl_part + (static_cast<size_t>(blockIdx.x) * 2 + (state & 4 ? 0 : 1)) * kCWarps * HEADS * kPartRow;
     st.template store<kPartRow>(slot_base + warp * HEADS * kPartRow, lane, g);
     const long long total = meta[0];
     const int n_ctas = meta[1];
@@ -722,77 +723,55 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(c
   extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hs = warp % U, rr = warp / U;      // head of the unit, token sub-row
-  WarpState &ws = reinterpret_cast<WarpState *>(smem + S::kWarp)[warp];
   int *meta = reinterpret_cast<int *>(smem + S::kMeta);
+  int *prefix = meta + 4, *lens = prefix + p.batch + 1;
+  PieceRec *rec = reinterpret_cast<PieceRec *>(smem + S::kPiece);
   const uint32_t full0 = smem_u32(smem + S::kBars), empty0 = full0 + 8 * C::kStages;
   const int g = p.h / p.kvh, slabs = p.kvh / U;
-  {
-    int *prefix = meta + 4, *lens = prefix + p.batch + 1;
-    const bool cache_bases = p.batch <= kBaseCacheMaxBatch4;
-    unsigned long long *bases = reinterpret_cast<unsigned long long *>(meta + meta_ints4(p.batch));
-    if (threadIdx.x < 32)   // K row's part, K scales, V rows 2 c4 and 2 c4 + 1 (without the lane's 8 bytes)
-      reinterpret_cast<int4 *>(smem + S::kAt)[lane] =
-          make_int4(token_of_row<U>(lane >> 2) * UB + 16 * (lane & 3), token_of_row<U>(lane >> 2) * UB,
-                    token_of_row<U>(2 * (lane & 3)) * UB, token_of_row<U>(2 * (lane & 3) + 1) * UB);
-    if (threadIdx.x == 0) {
-      for (int s = 0; s < C::kStages; ++s) {
-        mbar_init(full0 + 8 * s, kCWarps);
-        mbar_init(empty0 + 8 * s, kCWarps);
-      }
-      mbar_fence_init();
+  if (threadIdx.x < 32)   // K row's part, K scales, V rows 2 c4 and 2 c4 + 1 (without the lane's 8 bytes)
+    reinterpret_cast<int4 *>(smem + S::kAt)[lane] =
+        make_int4(token_of_row<U>(lane >> 2) * UB + 16 * (lane & 3), token_of_row<U>(lane >> 2) * UB,
+                  token_of_row<U>(2 * (lane & 3)) * UB, token_of_row<U>(2 * (lane & 3) + 1) * UB);
+  if (threadIdx.x == 32) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, kCWarps);
     }
-    for (int i = threadIdx.x; i < p.batch; i += kThreads4) {
-      int len = max(p.seq_lens[i], 0);
-      if constexpr (LOG) len = min(len, p.logit_rows);   // the logits have room for no more
-      lens[i] = len;
-      prefix[i + 1] = len > 0 ? ((len + TOK - 1) / TOK + kBoundaryCost) * slabs : 0;
-      if (cache_bases) {
-        const int64_t slot = p.slot_ids[i];
-        bases[i] = p.k_table[slot];
-        bases[p.batch + i] = p.v_table[slot];
-      }
-    }
-    __syncthreads();
-    if (warp == 0) {
-      int carry = 0;
-      for (int base = 0; base < p.batch; base += 32) {
-        const int i = base + lane;
-        int v = i < p.batch ? prefix[i + 1] : 0;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const int n = __shfl_up_sync(0xffffffffu, v, off);
-          if (lane >= off) v += n;
-        }
-        if (i < p.batch) prefix[i + 1] = carry + v;
-        carry += __shfl_sync(0xffffffffu, v, 31);
-      }
-      if (lane == 0) {
-        prefix[0] = 0;
-        const int n_ctas = min(static_cast<int>(gridDim.x), carry);
-        const bool active = static_cast<int>(blockIdx.x) < n_ctas;
-        meta[0] = carry;
-        meta[1] = n_ctas;
-        meta[2] = active ? static_cast<int>(static_cast<long long>(carry) * (blockIdx.x + 1) / n_ctas) : 0;
-      }
-    }
-    __syncthreads();
-    if (lane == 0) {
-      const int n_ctas = meta[1];
-      ws.tau = static_cast<int>(blockIdx.x) < n_ctas ? static_cast<int>(static_cast<long long>(meta[0]) * blockIdx.x / n_ctas) : 0;
-      ws.pieces = ws.copy_piece = 0;
-    }
-    __syncwarp();
-    look_ahead<UB>(p, ws, meta, slabs, 0, lane);
-    if (lane == 0) ws.copy_tile = ws.piece[0].tile_begin;
-    __syncwarp();
+    mbar_fence_init();
   }
+  for (int i = threadIdx.x; i < p.batch; i += kThreads4) {
+    int len = max(p.seq_lens[i], 0);
+    if constexpr (LOG) len = min(len, p.logit_rows);   // the logits have room for no more
+    lens[i] = len;
+    prefix[i + 1] = len > 0 ? ((len + TOK - 1) / TOK + kBoundaryCost) * slabs : 0;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int carry = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+      const int i = base + lane;
+      int v = i < p.batch ? prefix[i + 1] : 0;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, v, off);
+        if (lane >= off) v += n;
+      }
+      if (i < p.batch) prefix[i + 1] = carry + v;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) {
+      prefix[0] = 0;
+      const int n_ctas = min(static_cast<int>(gridDim.x), carry);
+      meta[0] = carry;
+      meta[1] = n_ctas;
+      meta[3] = static_cast<int>(blockIdx.x) < n_ctas ? static_cast<int>(static_cast<long long>(carry) * blockIdx.x / n_ctas) : 0;
+    }
+  }
+  __syncthreads();
   pdl_launch_dependents();
-
-  bool failed = false;
-  for (int n = 0; n < C::kStages - 1; ++n) failed |= fetch_tile<U>(p, smem, ws, n, slabs, warp, lane, true) < 0;
+  const int end = static_cast<int>(blockIdx.x) < meta[1] ? static_cast<int>(static_cast<long long>(meta[0]) * (blockIdx.x + 1) / meta[1]) : 0;
 
   if (blockIdx.x == 0) {   // sequences without context produce zeros; nobody owns a tile of theirs
-    const int *prefix = meta + 4;
     for (int b = 0; b < p.batch; ++b)
       if (prefix[b + 1] == prefix[b]) {
         for (int i = threadIdx.x; i < p.h * kHeadDim; i += kThreads4)
@@ -801,25 +780,42 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(c
           for (int i = threadIdx.x; i < p.h; i += kThreads4) p.lse[b * p.h + i] = -INFINITY;
       }
   }
-  int it = 0;
-  for (int now = 0; now < ws.pieces; ++now) {
-    if (now > 0) look_ahead<UB>(p, ws, meta, slabs, now, lane);
-    const PieceRec &pc = ws.piece[now % kPieces];
-    if (p.overlap == 2) pdl_wait_prior_grid();
-    const int64_t append_off = p.new_key ? p.byte_off[pc.b] : -1;
-    const bool fresh = append_off >= 0 && pc.tile_end == pc.tiles && ((pc.seq_len - 1) % TOK / 16) % R == rr;
-    if (fresh) append_row<U>(p, ws, pc, hs, append_off, lane);   // this warp owns the newest token's row of its head
-    const int got = run_piece<U, NB, LOG>(p, now, it, failed, fresh);
-    failed = got & 1;
-    it += pc.tile_end - pc.tile_begin;
-    if (got & 2) {
-      const long long total = meta[0];
-      const int n_ctas = meta[1];
-      merge_head<U, R, HEADS>(p, pc.b, pc.slab * U + hs, pc.stream_begin, total, n_ctas, owner_of(pc.stream_begin + kBoundaryCost, total, n_ctas),
-                              owner_of(pc.stream_end - 1, total, n_ctas), lane, g);
+  bool failed = false, first = true, more = true;
+  int it = 0;   // tiles of the share so far
+  while (more) {
+    if (warp == 0) look_up<UB>(p, rec, meta, slabs, end, lane);
+    __syncthreads();
+    const int pieces = meta[2];
+    int copy_piece = 0, copy_tile = rec[0].tile_begin;
+    const int ahead = (warp - it) & (kCWarps - 1);   // warp n % 8 fetches tile n
+    next_copy(rec, pieces, copy_piece, copy_tile, ahead);
+    if (ahead < C::kStages - 1 && copy_piece < pieces) {
+      const int n = it + ahead;
+      failed |= fetch_tile<U>(p, smem, rec[copy_piece], copy_tile, n % C::kStages, n / C::kStages, slabs, lane, true) < 0;
+      next_copy(rec, pieces, copy_piece, copy_tile, kCWarps);
     }
-    // a stream that lies wholly in this CTA's share used slot 1, as the next piece may
-    if (R > 1 && pc.tile_begin == 0 && pc.tile_end == pc.tiles) named_bar_sync(1, kCWarps * 32);
+    for (int now = 0; now < pieces; ++now) {
+      const PieceRec &pc = rec[now];
+      if (p.overlap == 2) pdl_wait_prior_grid();
+      const int64_t append_off = p.new_key ? p.byte_off[pc.b] : -1;
+      const bool fresh = append_off >= 0 && pc.tile_end == pc.tiles && ((pc.seq_len - 1) % TOK / 16) % R == rr;
+      if (fresh)   // this warp owns the newest token's row of its head
+        append_row<U>(p, reinterpret_cast<FreshRow *>(smem + S::kFresh)[warp], pc, hs, append_off, lane);
+      const int got = run_piece<U, NB, LOG>(p, now, it, (failed ? 1 : 0) | (fresh ? 2 : 0) | (first ? 4 : 0), copy_piece, copy_tile);
+      failed = got & 1;
+      first = false;
+      it += pc.tile_end - pc.tile_begin;
+      if (got & 2) {
+        const long long total = meta[0];
+        const int n_ctas = meta[1];
+        merge_head<U, R, HEADS>(p, pc.b, pc.slab * U + hs, pc.stream_begin, total, n_ctas,
+                                owner_of(pc.stream_begin + kBoundaryCost, total, n_ctas), owner_of(pc.stream_end - 1, total, n_ctas), lane, g);
+      }
+      // a stream that lies wholly in this CTA's share used slot 1, as the next piece may
+      if (R > 1 && pc.tile_begin == 0 && pc.tile_end == pc.tiles) named_bar_sync(1, kCWarps * 32);
+    }
+    more = meta[3] < end;
+    __syncthreads();   // the list and its end are read no more
   }
 }
 

@@ -85,6 +85,28 @@ def test_decode_attention_long_and_many(h, kvh, batch, hi):
     check_attention(r, q, out.cpu(), None, 128 ** -0.5)
 
 
+def test_more_pieces_than_a_share_lists_at_once():
+    """A thousand contexts of 1 to 5 rows over 128 kv heads: about 54 one-tile streams per CTA."""
+    from glake_b200 import ops
+    h = kvh = 128
+    rs = np.random.RandomState(0)
+    lens = [int(x) for x in rs.randint(1, 6, size=1000)]
+    k, v, ks, vs, rs = make(1, lens, kvh)
+    r = U.Ranges(k, v, "int4", ks, vs)
+    q = normal_bf16(rs, len(lens), h, 128)
+    out = torch.empty(len(lens), h, 128, dtype=torch.bfloat16, device="cuda")
+    ops.paged_attention_v1(out, q.cuda(), r.k_table.data_ptr(), r.v_table.data_ptr(), kvh, 128 ** -0.5, r.seq_lens, 1, r.max_len,
+                           None, "int4", 1.0, r.slot_ids, k_scale=ks.cuda(), v_scale=vs.cuda())
+    torch.cuda.synchronize()
+    assert ops.attn_status() == 0
+    for i in range(0, len(lens), 7):
+        kk, vv = r.rows64("k", i), r.rows64("v", i)
+        want, _, _, mag = U.attention64(q[i], kk, vv, 128 ** -0.5)
+        e = U.logit_error(q[i], kk, 128 ** -0.5, "int4")
+        tol = want.abs() * 2.0 ** -8 + mag * (2.0 ** -10 + 2 * e) + v_step(r, i, h) * 2.0 ** -13
+        assert bool(((out[i].cpu().double() - want).abs() <= tol).all())
+
+
 def test_small_and_large_magnitudes():
     """Queries far from 1, values whose scales differ by 2^60 between heads, one-sided logits of several hundred."""
     from glake_b200 import ops

@@ -53,16 +53,11 @@ __device__ __forceinline__ bool codes_fast(const float (&x)[16], float step, uin
   }
   return worst < 0.49999f && !(step > 0.f && step < 1.18e-38f);
 }
-__device__ __noinline__ void codes_exact(const float *x, float step, uint32_t *c) {
-  for (int i = 0; i < 4; ++i) {
-    c[i] = 0;
-    for (int j = 0; j < 4; ++j) {
-      const float v = x[4 * i + j];
-      int q = 0;
-      if (step > 0.f && v == v) q = static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(v, step)), -7.f), 7.f));
-      c[i] |= static_cast<uint32_t>(q + 8) << (4 * j);
-    }
-  }
+// The code of one element, by definition.  (By value: an array handed over would live in local memory in every round.)
+__device__ __noinline__ uint32_t code_exact(float x, float step) {
+  int q = 0;
+  if (step > 0.f && x == x) q = static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(x, step)), -7.f), 7.f));
+  return static_cast<uint32_t>(q + 8);
 }
 
 // Eight lanes per (row, kv head, K or V): lane 2 G + p brings dims 32 G + 16 p .. + 15, i.e. the codes of group G for
@@ -84,22 +79,36 @@ __global__ void __launch_bounds__(kThreads) append_int4_kernel(AppendParams p, i
   const uint32_t items = static_cast<uint32_t>(t1 - t0) * p.kvh * 2;
   char *const base[2] = {reinterpret_cast<char *>(p.k_table[slot]) + off, reinterpret_cast<char *>(p.v_table[slot]) + off};
   const int u = int4_unit(p.kvh), ub = int4_unit_bytes(u), ushift = __ffs(u) - 1;
-  // whole warps go round together: lanes past the last item work on it again and do not store
-  for (uint32_t first = threadIdx.x / 32 * 4; first < items; first += kItems) {
-    const uint32_t mine = first + (lane >> 3), it = min(mine, items - 1);
-    const uint32_t rest = kvh_div.div(it);
-    const int head = it - rest * p.kvh, kv = rest & 1, t = t0 + (rest >> 1);
-    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(kv ? p.value : p.key) +
-                               (src0 + t) * (kv ? p.value_stride : p.key_stride) + head * kHeadDim + l8 * 16;
-    uint32_t w[8];
+  // A round's 32 bytes and head scale are loaded one round ahead.  Whole warps go round together: lanes past the last
+  // item work on it again and do not store.
+  struct Item { uint32_t w[8]; float head_scale; int head, kv, t; };
+  const auto load = [&](uint32_t first, Item &it) {
+    const uint32_t n = min(first + (lane >> 3), items - 1);
+    const uint32_t rest = kvh_div.div(n);
+    it.head = n - rest * p.kvh;
+    it.kv = rest & 1;
+    it.t = t0 + (rest >> 1);
+    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(it.kv ? p.value : p.key) +
+                               (src0 + it.t) * (it.kv ? p.value_stride : p.key_stride) + it.head * kHeadDim + l8 * 16;
     if (vec_ok) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4 *>(src)), b = __ldg(reinterpret_cast<const uint4 *>(src) + 1);
-      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+      const uint4 a = __ldcs(reinterpret_cast<const uint4 *>(src)), b = __ldcs(reinterpret_cast<const uint4 *>(src) + 1);
+      it.w[0] = a.x; it.w[1] = a.y; it.w[2] = a.z; it.w[3] = a.w; it.w[4] = b.x; it.w[5] = b.y; it.w[6] = b.z; it.w[7] = b.w;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        w[e] = __bfloat16_as_ushort(src[2 * e]) | static_cast<uint32_t>(__bfloat16_as_ushort(src[2 * e + 1])) << 16;
+        it.w[e] = __bfloat16_as_ushort(src[2 * e]) | static_cast<uint32_t>(__bfloat16_as_ushort(src[2 * e + 1])) << 16;
     }
+    it.head_scale = __ldg((it.kv ? p.v_scale : p.k_scale) + it.head);
+  };
+  Item next;
+  uint32_t first = threadIdx.x / 32 * 4;
+  if (first < items) load(first, next);
+  for (; first < items; first += kItems) {
+    const Item cur = next;
+    if (first + kItems < items) load(first + kItems, next);
+    const uint32_t(&w)[8] = cur.w;
+    const int head = cur.head, kv = cur.kv, t = cur.t;
+    const uint32_t mine = first + (lane >> 3);
     float x[16];
 #pragma unroll
     for (int e = 0; e < 8; ++e) { x[2 * e] = bf16_lo(w[e]); x[2 * e + 1] = bf16_hi(w[e]); }
@@ -114,13 +123,18 @@ __global__ void __launch_bounds__(kThreads) append_int4_kernel(AppendParams p, i
       for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[e]));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     }
-    const float head_scale = (kv ? p.v_scale : p.k_scale)[head];
+    const float head_scale = cur.head_scale;
     uint32_t s8 = float2_to_e4m3x2(__fdiv_rn(amax, __fmul_rn(7.0f, head_scale)), 0.f) & 0xffu;
     const float step = __fmul_rn(e4m3_to_float(s8), head_scale);
     if (!(step > 0.f)) s8 = 0u;
     uint32_t c[4];
     const bool sure = codes_fast(x, step, c);
-    if (odd || !sure || s8 >= 0x7eu) codes_exact(x, step, c);   // NaN, a near tie, a saturated scale
+    if (odd || !sure || s8 >= 0x7eu) {   // NaN, a near tie, a saturated scale
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        c[e] = code_exact(x[4 * e], step) | code_exact(x[4 * e + 1], step) << 4 | code_exact(x[4 * e + 2], step) << 8 |
+               code_exact(x[4 * e + 3], step) << 12;
+    }
     // transposition: word of group G, piece i -> words of piece G
     const uint32_t a = __byte_perm(c[0], c[1], 0x5410), b = __byte_perm(c[2], c[3], 0x5410);
     const bool upper = (G & 2) != 0, odd_group = (G & 1) != 0;
@@ -164,41 +178,60 @@ __global__ void __launch_bounds__(kThreads) dequant_kernel(KvDequantParams p, in
     if (!out) continue;
     const char *base = reinterpret_cast<const char *>(kv ? p.v_table[slot] : p.k_table[slot]);
     const float *scale = kv ? p.v_scale : p.k_scale;
-#pragma unroll 2
-    for (uint32_t it = threadIdx.x >> 3; it < items; it += kItems) {
-      const uint32_t r = kvh_div.div(it);
-      const int head = it - r * p.kvh, t = t0 + r;
-      const char *row = base + t * row_bytes;
-      const float sc = __ldg(scale + head);
-      __nv_bfloat16 *dst = out + ((out0 + t) * p.kvh + head) * kHeadDim;
+    struct Item { uint4 w; uint32_t sw; float sc; uint32_t r; int head; };
+    const auto load = [&](uint32_t n, Item &it) {
+      it.r = kvh_div.div(n);
+      it.head = n - it.r * p.kvh;
+      const char *row = base + (t0 + static_cast<int>(it.r)) * row_bytes;
       if constexpr (INT4) {
-        const char *unit = row + (head >> ushift) * ub;
-        const int hh = head & (u - 1);
-        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(unit + hh * 64) + l8);   // piece l8: four dims of every group
-        const uint32_t sw = __ldg(reinterpret_cast<const uint32_t *>(unit + 64 * u) + hh);
-        float s8[4];
-        e4m3x4_to_float(sw, s8);
-#pragma unroll
-        for (int G = 0; G < 4; ++G) {
-          const uint32_t x = (G & 2 ? w.y : w.x) >> (16 * (G & 1));
-          float f[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {   // 2^23 + nibble as a float, less 2^23 + 8
-            const float q = __uint_as_float(((x >> (4 * j)) & 15u) | 0x4b000000u) - 8388616.f;
-            f[j] = __fmul_rn(q * s8[G], sc);
-          }
-          *reinterpret_cast<uint2 *>(dst + 32 * G + 4 * l8) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
-        }
+        const char *unit = row + (it.head >> ushift) * ub;
+        const int hh = it.head & (u - 1);
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(unit + hh * 64) + l8);   // piece l8: four dims of every group
+        it.w = make_uint4(w.x, w.y, 0, 0);
+        it.sw = __ldg(reinterpret_cast<const uint32_t *>(unit + 64 * u) + hh);
       } else {
-        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(row + head * kHeadDim) + l8);
-        float f[16];
-        Unpack<true>::run(w, f);
-        uint32_t o[8];
+        it.w = __ldcs(reinterpret_cast<const uint4 *>(row + it.head * kHeadDim) + l8);
+      }
+      it.sc = __ldg(scale + it.head);
+    };
+    // two items a round, the next round's in flight
+    constexpr int N = 2;
+    Item next[N];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = pack_bf16(__fmul_rn(f[2 * j], sc), __fmul_rn(f[2 * j + 1], sc));
-        uint4 *q = reinterpret_cast<uint4 *>(dst + 16 * l8);
-        q[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        q[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    for (int k = 0; k < N; ++k)
+      if ((threadIdx.x >> 3) + k * kItems < items) load((threadIdx.x >> 3) + k * kItems, next[k]);
+    for (uint32_t first = threadIdx.x >> 3; first < items; first += N * kItems) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const uint32_t n = first + k * kItems;
+        if (n >= items) break;
+        const Item cur = next[k];
+        if (n + N * kItems < items) load(n + N * kItems, next[k]);
+        __nv_bfloat16 *dst = out + ((out0 + t0 + static_cast<int>(cur.r)) * p.kvh + cur.head) * kHeadDim;
+        if constexpr (INT4) {
+          float s8[4];
+          e4m3x4_to_float(cur.sw, s8);
+#pragma unroll
+          for (int G = 0; G < 4; ++G) {
+            const uint32_t x = (G & 2 ? cur.w.y : cur.w.x) >> (16 * (G & 1));
+            float f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {   // 2^23 + nibble as a float, less 2^23 + 8
+              const float q = __uint_as_float(((x >> (4 * j)) & 15u) | 0x4b000000u) - 8388616.f;
+              f[j] = __fmul_rn(q * s8[G], cur.sc);
+            }
+            *reinterpret_cast<uint2 *>(dst + 32 * G + 4 * l8) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
+          }
+        } else {
+          float f[16];
+          Unpack<true>::run(cur.w, f);
+          uint32_t o[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = pack_bf16(__fmul_rn(f[2 * j], cur.sc), __fmul_rn(f[2 * j + 1], cur.sc));
+          uint4 *q = reinterpret_cast<uint4 *>(dst + 16 * l8);
+          q[0] = make_uint4(o[0], o[1], o[2], o[3]);
+          q[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        }
       }
     }
   }

@@ -8,7 +8,7 @@
 // select_kernel: one CTA per (sequence, kv head).  Radix selection (11 + 11 + 10 bits of the order-preserving integer
 //   of the weight) finds the key of the last row that fits and how many rows with that key do; then every warp walks
 //   its run of rows once, ranks by ballots and writes the kept row numbers and the compacted weights.  Weights are
-//   held in shared memory when they fit (49 152 rows), so memory sees them once; also what makes scores_out == scores safe.
+//   held in shared memory when they fit (45 056 rows), so memory sees them once; also what makes scores_out == scores safe.
 // move_kernel: a chunk of kept rows per CTA, through registers.  In place, a destination row may still be the source
 //   of an earlier destination (kept[i] >= i).  Chunks draw their number from a counter, load all their rows,
 //   raise a flag, and store after the flags of the earlier chunks of the same head whose sources reach into their
@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelSmemRows = 49152;
+constexpr int kSelSmemRows = 45056;   // with the ballots and the histogram: 201 KB
 constexpr int kMoveThreads = 256;
 constexpr uint32_t kNoKey = 0xffffffffu;
 
@@ -38,8 +38,12 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+constexpr int kSelList = 2048;
+
 struct SelectState {
   int hist[2048];
+  uint32_t list[kSelList];   // keys that share the first digit's prefix, when they are few
+  int listed;
   int warp_sum[kSelWarps];
   int warp_gt[kSelWarps], warp_eq[kSelWarps];
   uint32_t prefix;   // digits fixed so far
@@ -79,90 +83,105 @@ __device__ __forceinline__ void pick_digit(SelectState &st, int bins, int shift)
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(kSelThreads) select_kernel(EvictParams p) {
-  extern __shared__ __align__(16) float held[];
-  __shared__ SelectState st;
-  const int b = blockIdx.x / p.kvh, head = blockIdx.x % p.kvh;
+// The rows to keep of one (sequence, head) with n > budget.  HELD: the weights are in shared memory (`held`, loaded here);
+// otherwise every pass reads them from memory again.  ballots: two words per 32 rows (above the limit | equal to it).
+template <bool HELD>
+__device__ __forceinline__ void select_rows(const EvictParams &p, SelectState &st, float *held, uint2 *ballots, const float *src, float *dst,
+                                            int32_t *kept, int n) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n = min(max(p.seq_lens[b], 0), p.max_seq_len);
-  const int64_t row0 = p.slot_ids[b] * p.slot_stride + head * p.head_stride;
-  const float *src = p.scores + row0;
-  float *dst = p.scores_out + row0;
-  int32_t *kept = p.kept + static_cast<int64_t>(blockIdx.x) * p.budget;
-  for (int c = tid; c < p.chunks; c += kSelThreads) p.flags[static_cast<int64_t>(blockIdx.x) * p.chunks + c] = 0;
-  if (blockIdx.x == 0 && tid == 0) *p.ticket = 0;
-  if (n <= p.budget) {   // everything stays
-    for (int t = tid; t < p.budget; t += kSelThreads) kept[t] = t < n ? t : -1;
-    if (src != dst)
-      for (int t = tid; t < n; t += kSelThreads) dst[t] = src[t];
-    return;
-  }
-  const bool in_smem = n <= p.held_rows;
   const int lo = p.sink, hi = n - p.recent;   // rows that may go
   const int need = p.budget - p.sink - p.recent;
-  if (in_smem)
-    for (int t = tid; t < n; t += kSelThreads) held[t] = __ldcg(src + t);
-  if (tid == 0) { st.prefix = 0; st.want = need; }
-  const auto weight = [&](int t) { return in_smem ? held[t] : __ldcg(src + t); };
+  const auto weight = [&](int t) { return HELD ? held[t] : __ldcg(src + t); };
+  for (int i = tid; i < 2048; i += kSelThreads) st.hist[i] = 0;
+  if (tid == 0) { st.prefix = 0; st.want = need; st.listed = 0; }
+  __syncthreads();
+  // the weights come in and the first digit (sign, exponent, two bits) is counted on the way
+#pragma unroll 4
+  for (int t = tid; t < n; t += kSelThreads) {
+    const float x = __ldcg(src + t);
+    if (HELD) held[t] = x;
+    if (t >= lo && t < hi) atomicAdd(&st.hist[weight_key(x) >> 21], 1);
+  }
+  __syncthreads();
   uint32_t limit = kNoKey;   // rows with a key above stay; `ties` of those equal to it
   int ties = 0;
   if (need > 0) {
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-      const int bins = pass == 2 ? 1024 : 2048;
-      const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-      for (int i = tid; i < bins; i += kSelThreads) st.hist[i] = 0;
-      __syncthreads();
-      const uint32_t prefix = st.prefix;
+    pick_digit(st, 2048, 21);
+    for (int i = tid; i < 2048; i += kSelThreads) st.hist[i] = 0;
+    const uint32_t first = st.prefix;
+    __syncthreads();
+#pragma unroll 4
+    for (int t = lo + tid; t < hi; t += kSelThreads) {
+      const uint32_t key = weight_key(weight(t));
+      if ((key & 0xffe00000u) == first) {
+        atomicAdd(&st.hist[(key >> 10) & 2047u], 1);
+        const int at = atomicAdd(&st.listed, 1);
+        if (at < kSelList) st.list[at] = key;
+      }
+    }
+    __syncthreads();
+    pick_digit(st, 2048, 10);
+    for (int i = tid; i < 1024; i += kSelThreads) st.hist[i] = 0;
+    const uint32_t second = st.prefix;
+    const int listed = st.listed;
+    __syncthreads();
+    if (listed <= kSelList) {
+      for (int i = tid; i < listed; i += kSelThreads)
+        if ((st.list[i] & 0xfffffc00u) == second) atomicAdd(&st.hist[st.list[i] & 1023u], 1);
+    } else {
+#pragma unroll 4
       for (int t = lo + tid; t < hi; t += kSelThreads) {
         const uint32_t key = weight_key(weight(t));
-        if ((key & mask) == prefix) atomicAdd(&st.hist[(key >> shift) & (bins - 1)], 1);
+        if ((key & 0xfffffc00u) == second) atomicAdd(&st.hist[key & 1023u], 1);
       }
-      __syncthreads();
-      pick_digit(st, bins, shift);
     }
+    __syncthreads();
+    pick_digit(st, 1024, 0);
     limit = st.prefix;
     ties = st.want;
   }
-  __syncthreads();
-  // every warp owns a run of rows; count, scan over the warps, then write
+  // Every warp owns a run of rows: count by ballots (kept in shared memory while there is room), scan over the warps, write.
   const int run = (n + kSelThreads - 1) / kSelThreads * 32;
   const int r0 = min(warp * run, n), r1 = min(r0 + run, n);
-  const auto rank = [&](int t, bool *stays, bool *tie) {
-    *stays = *tie = false;
-    if (t >= r1) return;
-    if (t < lo || t >= hi) { *stays = true; return; }
-    if (need <= 0) return;
-    const uint32_t key = weight_key(weight(t));
-    *stays = key > limit;
-    *tie = key == limit;
+  const auto rank = [&](int t) {
+    bool stays = false, tie = false;
+    if (t < r1) {
+      if (t < lo || t >= hi) {
+        stays = true;
+      } else if (need > 0) {
+        const uint32_t key = weight_key(weight(t));
+        stays = key > limit;
+        tie = key == limit;
+      }
+    }
+    return make_uint2(__ballot_sync(0xffffffffu, stays), __ballot_sync(0xffffffffu, tie));
   };
   int gt = 0, eq = 0;
+#pragma unroll 4
   for (int t = r0; t < r1; t += 32) {
-    bool s, e;
-    rank(t + lane, &s, &e);
-    gt += __popc(__ballot_sync(0xffffffffu, s));
-    eq += __popc(__ballot_sync(0xffffffffu, e));
+    const uint2 b = rank(t + lane);
+    if (HELD && lane == 0) ballots[t >> 5] = b;
+    gt += __popc(b.x);
+    eq += __popc(b.y);
   }
   if (lane == 0) { st.warp_gt[warp] = gt; st.warp_eq[warp] = eq; }
   __syncthreads();
   gt = eq = 0;
   for (int w = 0; w < warp; ++w) { gt += st.warp_gt[w]; eq += st.warp_eq[w]; }
-  const bool write_now = in_smem || src != dst;
+  const bool write_now = HELD || src != dst;
+  const unsigned below = (1u << lane) - 1u;
+#pragma unroll 4
   for (int t = r0; t < r1; t += 32) {
-    bool s, e;
-    rank(t + lane, &s, &e);
-    const unsigned bs = __ballot_sync(0xffffffffu, s), be = __ballot_sync(0xffffffffu, e);
-    const unsigned below = (1u << lane) - 1u;
-    const int my_eq = eq + __popc(be & below);
+    const uint2 b = HELD ? ballots[t >> 5] : rank(t + lane);
+    const bool s = (b.x >> lane) & 1u, e = (b.y >> lane) & 1u;
+    const int my_eq = eq + __popc(b.y & below);
     if (s || (e && my_eq < ties)) {
-      const int at = gt + __popc(bs & below) + min(my_eq, ties);
+      const int at = gt + __popc(b.x & below) + min(my_eq, ties);
       kept[at] = t + lane;
       if (write_now) dst[at] = weight(t + lane);
     }
-    gt += __popc(bs);
-    eq += __popc(be);
+    gt += __popc(b.x);
+    eq += __popc(b.y);
   }
   __syncthreads();
   if (!write_now) {
@@ -177,6 +196,30 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(EvictParams p) {
     }
   }
   for (int t = p.budget + tid; t < n; t += kSelThreads) dst[t] = 0.f;
+}
+
+__global__ void __launch_bounds__(kSelThreads) select_kernel(EvictParams p) {
+  extern __shared__ __align__(16) float held[];
+  __shared__ SelectState st;
+  const int b = blockIdx.x / p.kvh, head = blockIdx.x % p.kvh, tid = threadIdx.x;
+  const int n = min(max(p.seq_lens[b], 0), p.max_seq_len);
+  const int64_t row0 = p.slot_ids[b] * p.slot_stride + head * p.head_stride;
+  const float *src = p.scores + row0;
+  float *dst = p.scores_out + row0;
+  int32_t *kept = p.kept + static_cast<int64_t>(blockIdx.x) * p.budget;
+  for (int c = tid; c < p.chunks; c += kSelThreads) p.flags[static_cast<int64_t>(blockIdx.x) * p.chunks + c] = 0;
+  if (blockIdx.x == 0 && tid == 0) *p.ticket = 0;
+  if (n <= p.budget) {   // everything stays
+    for (int t = tid; t < p.budget; t += kSelThreads) kept[t] = t < n ? t : -1;
+    if (src != dst)
+      for (int t = tid; t < n; t += kSelThreads) dst[t] = src[t];
+    return;
+  }
+  uint2 *ballots = reinterpret_cast<uint2 *>(held + (p.held_rows + 3) / 4 * 4);
+  if (n <= p.held_rows)
+    select_rows<true>(p, st, held, ballots, src, dst, kept, n);
+  else
+    select_rows<false>(p, st, held, ballots, src, dst, kept, n);
 }
 
 // VEC 16-byte vectors of a row and head: 16 bf16, 8 fp8, 4 for the 4-bit cache, which has a 4-byte scale word beside.
@@ -280,7 +323,7 @@ int launch_evict(const EvictParams &p_in, int kv_dtype, cudaStream_t stream) {
   EvictParams p = p_in;
   p.held_rows = std::min(p.max_seq_len, kSelSmemRows);
   static SmemOptIn opt_in;
-  const int smem = p.held_rows * static_cast<int>(sizeof(float));
+  const int smem = (p.held_rows + 3) / 4 * 16 + (p.held_rows / 32 + 1) * static_cast<int>(sizeof(uint2));
   if (!opt_in.ensure(select_kernel, smem)) return VT_ERR_CUDA;
   const int heads = p.batch * p.kvh;
   select_kernel<<<heads, kSelThreads, smem, stream>>>(p);

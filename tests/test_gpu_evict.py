@@ -97,7 +97,7 @@ def test_weights_and_windows(kind, budget, sink, recent):
 @pytest.mark.parametrize("in_place", [True, False])
 def test_rows_beyond_shared_memory(in_place):
     """More rows than the selection holds on chip: weights are read again, and moved in order when in place."""
-    Case([60000, 49153, 49152, 10], 1, "fp8_e4m3", 5, "ties").check(20000, 4, 100, in_place)
+    Case([60000, 45057, 45056, 10], 1, "fp8_e4m3", 5, "ties").check(20000, 4, 100, in_place)
 
 
 @pytest.mark.parametrize("kv", ["bf16", "fp8_e4m3", "int4"])

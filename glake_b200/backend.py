@@ -315,16 +315,19 @@ class DecodeRunner:
     BUCKET = 2048  # graphs are keyed by max context rounded up to this many tokens
 
     def __init__(self, engine: VTensorCacheEngine, impl: VTensorAttentionImpl, batch, host_io=False,
-                 k_scale=None, v_scale=None, overlap=True, post_layer=None, launches_per_post_layer=0):
+                 k_scale=None, v_scale=None, overlap=True, post_layer=None, launches_per_post_layer=0, scores=None):
         """``post_layer(layer)``, when given, is called on the runner's stream after every
         layer's attention, inside the captured graph: the place of what the model does
         between two attention layers, e.g. the tensor-parallel all-reduces after o_proj
-        and down_proj (GLakeServe/vllm/model_executor/layers/linear.py:690-691)."""
+        and down_proj (GLakeServe/vllm/model_executor/layers/linear.py:690-691).
+        ``scores`` (``VTensorCacheEngine.new_scores``) accumulates every layer's attention weights; the
+        layers' launches do not overlap then."""
         self.engine, self.impl, self.batch, self.host_io = engine, impl, batch, host_io
         self.post_layer, self.launches_per_post_layer = post_layer, launches_per_post_layer
         self.prepare_seconds = []     # host time of the allocator bookkeeping of each step
         # consecutive layers touch disjoint ranges: let layer l+1 start as layer l drains
-        self.overlap = overlap and engine.num_layers > 1
+        self.overlap = overlap and engine.num_layers > 1 and scores is None
+        self.scores = scores
         self.k_scale, self.v_scale = k_scale, v_scale
         dev, layers = engine.device, engine.num_layers
         hd, kd = impl.num_heads * impl.head_size, impl.num_kv_heads * impl.head_size
@@ -399,7 +402,8 @@ class DecodeRunner:
                             self.v[layer], kc.vmm_ptr, vc.vmm_ptr, self.d64[:b], self.d64[b:], self.d32[:b],
                             meta.max_seq_len, self.impl.num_kv_heads, self.impl.scale, self.impl.kv_cache_dtype,
                             ks, vs, overlap=self._overlap_mode(layer), workspace=self.workspace,
-                            maps=self.engine.decode_maps(layer, self.impl.num_heads), clean_scratch=True)
+                            maps=self.engine.decode_maps(layer, self.impl.num_heads), clean_scratch=True,
+                            scores=self.scores[layer] if self.scores is not None else None)
             torch.cuda.nvtx.range_pop()
             if self.post_layer is not None:
                 self.post_layer(layer)
@@ -448,9 +452,15 @@ class DecodeRunner:
                 self.staged[cur] = torch.cuda.Event(blocking=True)
             self.staged[cur].record(self.stream)
         bucket = (meta.max_seq_len + self.BUCKET - 1) // self.BUCKET * self.BUCKET
+        if self.scores is not None:
+            rows = self.scores[0].shape[2]
+            if meta.max_seq_len > rows:
+                raise RuntimeError(f"DecodeRunner: a context of {meta.max_seq_len} rows, scores hold {rows}")
+            bucket = min(bucket, rows)
         graph = self.graphs.get(bucket)
         if graph is None:
-            need = ops.new_workspace(self.engine.device, b, self.impl.num_heads, self.impl.head_size, bucket)
+            need = ops.new_workspace(self.engine.device, b, self.impl.num_heads, self.impl.head_size, bucket,
+                                     scored=self.scores is not None)
             if self.workspace is None or self.workspace.numel() < need.numel():
                 self.stream.synchronize()
                 self.workspace = need
@@ -471,7 +481,7 @@ class DecodeRunner:
                                               self.impl.kv_cache_dtype)
             # fused step: one kernel per layer; otherwise append + attention (+ merge)
             fused = variant == 2 and ops.step_is_fused(self.impl.kv_cache_dtype)
-            per_layer = 1 if fused else 2 + (1 if parts > 1 else 0)
+            per_layer = (1 if fused else 2 + (1 if parts > 1 else 0)) + (1 if self.scores is not None else 0)
             self.kernel_launches_per_step = self.engine.num_layers * (per_layer + self.launches_per_post_layer)
             return  # the warm-up pass above already executed this step
         with torch.cuda.stream(self.stream):

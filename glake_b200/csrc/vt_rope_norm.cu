@@ -23,6 +23,7 @@
 // residual stream when fused.
 #include "../../include/vtensor.h"
 #include "vt_device.cuh"
+#include "vt_int4.cuh"
 #include "vt_kernels.h"
 
 namespace vt {
@@ -175,6 +176,68 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(RopeParams p)
   }
 }
 
+// The same over a 4-bit cache: a group scale needs 32 neighbouring dims of the ROTATED key, so a warp takes one head of
+// one row (lane l: dims 4 l .. 4 l + 3), exchanges the NeoX pairs by shuffle and quantises from registers, from the
+// bf16-rounded key as a separate append would.  grid: (batch, row blocks).
+template <bool NEOX>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_int4_kernel(RopeParams p) {
+  const int i = blockIdx.x;
+  const bool decode = p.a.max_seq_len == 1;
+  const int n_rows = decode ? 1 : p.a.seq_lens[i];
+  const int t0 = blockIdx.y * kRopeRowsPerCta, t1 = min(t0 + kRopeRowsPerCta, n_rows);
+  const int64_t off = p.a.byte_off[i], slot = p.a.slot_ids[i];
+  const int kvh = p.a.kvh, heads = p.num_heads + 2 * kvh, half = p.rot_dim / 2;
+  const int64_t row_bytes = int4_row_bytes(kvh);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = 4 * lane;
+  for (int t = t0; t < t1; ++t) {
+    const int64_t src_row = decode ? i : static_cast<int64_t>(p.a.cache_seq_lens[i]) + t;
+    const __nv_bfloat16 *cs_row = p.cos_sin + p.positions[src_row] * p.rot_dim;
+    for (int w = warp; w < heads; w += kRopeThreads / 32) {
+      const bool is_q = w < p.num_heads, is_v = w >= p.num_heads + kvh;
+      const int head = is_q ? w : is_v ? w - p.num_heads - kvh : w - p.num_heads;
+      __nv_bfloat16 *hp = is_q ? p.query + src_row * p.query_stride + head * kHeadDim
+                        : is_v ? const_cast<__nv_bfloat16 *>(static_cast<const __nv_bfloat16 *>(p.a.value)) + src_row * p.a.value_stride + head * kHeadDim
+                               : p.key + src_row * p.a.key_stride + head * kHeadDim;
+      const uint2 raw = *reinterpret_cast<const uint2 *>(hp + d);
+      float x[4] = {bf16_lo(raw.x), bf16_hi(raw.x), bf16_lo(raw.y), bf16_hi(raw.y)};
+      if (!is_v) {
+        const bool rotated = d < p.rot_dim, upper = d >= half;
+        float o[4];
+        if constexpr (NEOX) {   // partner dims d + half (or d - half) sit half / 4 lanes away
+          const int from = rotated ? (upper ? lane - half / 4 : lane + half / 4) : lane;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = __shfl_sync(0xffffffffu, x[j], from);
+        }
+        if (rotated) {
+          const int c = NEOX ? (upper ? d - half : d) : d / 2;   // first cos / sin index of this lane
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (NEOX) {
+              const float cs = __bfloat162float(cs_row[c + j]), sn = __bfloat162float(cs_row[half + c + j]);
+              x[j] = upper ? __fmaf_rn(x[j], cs, __fmul_rn(o[j], sn)) : __fmaf_rn(x[j], cs, -__fmul_rn(o[j], sn));
+            } else if ((j & 1) == 0) {
+              const float cs = __bfloat162float(cs_row[c + j / 2]), sn = __bfloat162float(cs_row[half + c + j / 2]);
+              const float a = x[j], b = x[j + 1];
+              x[j] = __fmaf_rn(a, cs, -__fmul_rn(b, sn));
+              x[j + 1] = __fmaf_rn(b, cs, __fmul_rn(a, sn));
+            }
+          }
+        }
+        const uint2 out = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+        if (is_q || p.write_key) *reinterpret_cast<uint2 *>(hp + d) = out;
+        if (is_q) continue;
+        x[0] = bf16_lo(out.x); x[1] = bf16_hi(out.x); x[2] = bf16_lo(out.y); x[3] = bf16_hi(out.y);
+      }
+      if (off < 0) continue;   // padded entry: rotated, not appended
+      uint32_t bits, s8;
+      quantise4(x, (is_v ? p.a.v_scale : p.a.k_scale)[head], &bits, &s8);
+      char *row = reinterpret_cast<char *>(is_v ? p.a.v_table[slot] : p.a.k_table[slot]) + off + t * row_bytes;
+      *reinterpret_cast<uint16_t *>(row + int4_head_offset(kvh, head) + 8 * (lane & 7) + 2 * (lane >> 3)) = static_cast<uint16_t>(bits);
+      if ((lane & 7) == 0) row[int4_scale_offset(kvh, head) + (lane >> 3)] = static_cast<char>(s8);
+    }
+  }
+}
+
 // ---- RMS norm ------------------------------------------------------------
 constexpr int kNormThreads = 256;
 constexpr int kNormMaxVec = 8;    // 16-byte vectors a thread keeps: rows up to 256 * 8 * 8 = 16384 elements
@@ -257,8 +320,8 @@ int vt_rope_append(const int64_t *positions, void *query, int64_t query_stride, 
     return VT_ERR_INVALID;
   if (d != vt::kHeadDim) return VT_ERR_UNSUPPORTED;
   if (rot_dim <= 0 || rot_dim > d || rot_dim % 16 != 0) return VT_ERR_UNSUPPORTED;
-  if (kv_dtype != VT_KV_BF16 && kv_dtype != VT_KV_FP8_E4M3) return VT_ERR_UNSUPPORTED;
-  if (kv_dtype == VT_KV_FP8_E4M3 && (!k_scale || !v_scale)) return VT_ERR_INVALID;
+  if (kv_dtype != VT_KV_BF16 && kv_dtype != VT_KV_FP8_E4M3 && kv_dtype != VT_KV_INT4) return VT_ERR_UNSUPPORTED;
+  if (kv_dtype != VT_KV_BF16 && (!k_scale || !v_scale)) return VT_ERR_INVALID;
   if (max_seq_len > 1 && (!seq_lens || !cache_seq_lens)) return VT_ERR_INVALID;
   if (flags & ~VT_ROPE_WRITE_KEY) return VT_ERR_INVALID;
   if (query_stride < static_cast<int64_t>(num_heads) * d || key_stride < static_cast<int64_t>(kvh) * d ||
@@ -282,6 +345,11 @@ int vt_rope_append(const int64_t *positions, void *query, int64_t query_stride, 
   dim3 grid(batch, decode ? 1 : (max_seq_len + vt::kRopeRowsPerCta - 1) / vt::kRopeRowsPerCta);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool fp8 = kv_dtype == VT_KV_FP8_E4M3;
+  if (kv_dtype == VT_KV_INT4) {
+    if (is_neox) vt::rope_append_int4_kernel<true><<<grid, vt::kRopeThreads, 0, s>>>(p);
+    else vt::rope_append_int4_kernel<false><<<grid, vt::kRopeThreads, 0, s>>>(p);
+    return cudaGetLastError() == cudaSuccess ? VT_OK : VT_ERR_CUDA;
+  }
   if (fp8 && is_neox) vt::rope_append_kernel<true, true><<<grid, vt::kRopeThreads, 0, s>>>(p);
   else if (fp8) vt::rope_append_kernel<true, false><<<grid, vt::kRopeThreads, 0, s>>>(p);
   else if (is_neox) vt::rope_append_kernel<false, true><<<grid, vt::kRopeThreads, 0, s>>>(p);

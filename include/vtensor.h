@@ -469,7 +469,7 @@ int vt_prefill_attn_tma(void *out, int64_t out_stride, const void *q, int64_t q_
  *   the remaining arguments are vt_append's, with the same meaning; token row
  *   numbering (decode: row i; prefill: cache_seq_lens[i] + t) also indexes positions.
  * Arithmetic as the reference's CPU kernel (csrc/cpu/pos_encoding.cpp:23-89,
- * :109-166): fp32 products, one rounding to bf16; with an fp8 cache the rounded
+ * :109-166): fp32 products, one rounding to bf16; with an fp8 or 4-bit cache the rounded
  * bf16 key is what gets quantised, as in the two-kernel sequence.  Pointers must
  * be 16-byte aligned and strides multiples of 8 elements (VT_ERR_UNSUPPORTED). */
 #define VT_ROPE_WRITE_KEY 1u

@@ -288,6 +288,48 @@ def test_captured_and_replayed_on_another_stream():
     check_attention(r, q.cpu(), out.cpu(), None, 128 ** -0.5)
 
 
+@pytest.mark.parametrize("neox,rot", [(True, 128), (False, 128), (True, 64), (False, 32), (True, 16)])
+@pytest.mark.parametrize("h,kvh", [(8, 2), (4, 4), (16, 8), (3, 3)])
+@pytest.mark.parametrize("write_key", [False, True])
+def test_rope_append(neox, rot, h, kvh, write_key):
+    """One launch equals the rotation (bf16 cache, key written back) followed by the 4-bit append of the rotated key."""
+    from glake_b200 import ops
+    rs = np.random.RandomState(rot + h)
+    lens, n = [5, 1, 0, 33], 39
+    q, k, v = (normal_bf16(rs, n, x * 128).cuda() for x in (h, kvh, kvh))
+    pos = torch.from_numpy(rs.randint(0, 300, size=n)).cuda()
+    freq = torch.outer(torch.arange(300.0), 1.0 / 10000.0 ** (torch.arange(0, rot, 2) / rot))
+    cs = torch.cat([freq.cos(), freq.sin()], -1).bfloat16().cuda()
+    ks, vs = torch.rand(kvh) * 0.004 + 0.006, torch.rand(kvh) * 0.004 + 0.006
+    empty = [torch.zeros(x, kvh, 128, dtype=torch.bfloat16) for x in lens]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    starts, zero = i32([0, 5, 6, 6]), torch.zeros(4, dtype=torch.int64, device="cuda")
+    plain = U.Ranges(empty, empty, "bf16")
+    q0, k0 = q.clone(), k.clone()
+    ops.rotary_embedding_and_cache(pos, q0, k0, v, 128, cs, neox, plain.k_table, plain.v_table, zero, plain.slot_ids, i32(lens), starts, 33,
+                                   kvh, write_key=True)
+    r = U.Ranges(empty, empty, "int4", ks, vs)
+    before = r.k.clone()
+    q1, k1 = q.clone(), k.clone()
+    off = zero.clone()
+    off[1] = -1            # rotated, not appended
+    ops.rotary_embedding_and_cache(pos, q1, k1, v, 128, cs, neox, r.k_table, r.v_table, off, r.slot_ids, i32(lens), starts, 33, kvh, "int4",
+                                   ks.cuda(), vs.cuda(), write_key=write_key)
+    torch.cuda.synchronize()
+    assert torch.equal(q1, q0) and torch.equal(k1, k0 if write_key else k)
+    at = 0
+    for i, m in enumerate(lens):
+        for name, x, scale in (("k", k0, ks), ("v", v, vs)):
+            got = U.unpack4(getattr(r, name)[r.slots[i], :m].cpu(), kvh, scale)
+            want = U.unpack4(U.pack4(x[at:at + m].cpu().view(m, kvh, 128), scale), kvh, scale)
+            if i == 1:
+                assert torch.equal(getattr(r, name)[r.slots[i]], before[r.slots[i]])
+            else:
+                assert torch.equal(got, want)
+        assert bool((r.k[r.slots[i], m:] == 0xff).all())
+        at += m
+
+
 def test_backend_prompt_extend_and_decode():
     """Prompt, prefix-extend and decode through the engine's own ranges and VTensorAttentionImpl, two layers."""
     from glake_b200.backend import VTensorAttentionImpl, VTensorCacheEngine, VTensorMetadata, prepare_step

@@ -235,6 +235,54 @@ def test_capture_and_two_streams():
     assert torch.equal(c, want + want) and torch.equal(o, out)
 
 
+@pytest.mark.parametrize("kv", ["auto", "int4"])
+def test_decode_runner_accumulates(kv):
+    """Graph-replayed steps of two layers equal the same steps through the op, scores and cache rows included."""
+    from glake_b200 import ops
+    from glake_b200.backend import DecodeRunner, VTensorAttentionImpl, VTensorCacheEngine, VTensorMetadata
+    gpu_util.ensure_pool()
+    h, kvh, b = 8, 4, 3
+    scales = [torch.full((kvh,), 0.01, device="cuda")] * 2 if kv == "int4" else None
+    got = []
+    for graph in (True, False):
+        eng = VTensorCacheEngine(2, kvh, 128, b, 300, cache_dtype=kv)
+        try:
+            impl = VTensorAttentionImpl(h, 128, 0.1, kvh, kv)
+            scores = eng.new_scores(256)
+            rs = np.random.RandomState(3)
+            runner = DecodeRunner(eng, impl, b, k_scale=scales, v_scale=scales, scores=scores) if graph else None
+            outs = []
+            for step in range(5):
+                for s in eng.vmm_kvcache_segment:
+                    s.ensure_mapped((step + 1) * eng.token_size)
+                meta = VTensorMetadata(list(range(b)), [step + 1] * b, kvh, 128, num_decode_tokens=b)
+                ins = [[normal_bf16(rs, b, x * 128).cuda() for x in (h, kvh, kvh)] for _ in range(2)]
+                if graph:
+                    for layer, (q, k, v) in enumerate(ins):
+                        runner.q[layer].copy_(q), runner.k[layer].copy_(k), runner.v[layer].copy_(v)
+                    torch.cuda.synchronize()
+                    runner.step(meta)
+                    runner.synchronize()
+                    assert runner.status() == 0
+                    outs.append(runner.out.clone())
+                else:
+                    from glake_b200.backend import prepare_step
+                    prepare_step(meta, eng)
+                    outs.append(torch.stack([impl.forward(q, k, v, *eng.gpu_cache[layer], meta, k_scale=scales[layer] if scales else None,
+                                                          v_scale=scales[layer] if scales else None, scores=scores[layer])
+                                             for layer, (q, k, v) in enumerate(ins)]))
+                    torch.cuda.synchronize()
+            got.append((torch.stack(outs), torch.stack(scores)))
+            if graph:
+                with pytest.raises(RuntimeError, match="scores hold 256"):
+                    runner.step(VTensorMetadata([0, 1, 2], [257, 1, 1], kvh, 128, num_decode_tokens=3, set_used_size=[1, 1, 1]))
+        finally:
+            torch.cuda.synchronize()
+            eng.close()
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert bool(((got[0][1].sum((0, 2, 3)) - 5 * 2 * h).abs() < 1e-3).all())
+
+
 def test_backend_scores_and_evicts():
     """A prompt scored by its window, decode steps that accumulate, an eviction that gives chunks back, and more steps:
     every layer follows the plain computation on its own list of rows."""

@@ -186,7 +186,8 @@ int vt_pool_write(vt_pool *pool, uint64_t dst_dptr, const void *src_host, size_t
  *                 path; arithmetic follows csrc/quantization/fp8/nvidia/quant_utils.cuh:467-479);
  *                 VT_KV_INT4: per 32 dims of a head s = e4m3(amax / (7 scale[kv_head])),
  *                 saturating at 448, and q = clamp(round(x / (s scale[kv_head])), -7, 7), ties to
- *                 even; NaN is stored as 0 and infinities saturate; k_scale/v_scale as for fp8;
+ *                 even, each product and quotient rounded to fp32; NaN is stored as 0 and
+ *                 infinities saturate; k_scale/v_scale as for fp8;
  *                 row = vt_kv_row_bytes: every unit of U kv heads is U x 64 bytes, dim
  *                 32 G + 4 r + j in byte 8 r + 2 G + j / 2 (low nibble for even j) as q + 8, then
  *                 U x 4 bytes with the e4m3 scales of the groups G = 0..3, then padding to 16 bytes

@@ -138,7 +138,8 @@ def test_append_and_read_back(kvh, offset):
     key[0, 0, 3], key[0, 0, 40], key[1, 0, 70], value[2, 0, 5] = math.nan, math.inf, 0.0, -math.inf
     key[3] = 0
     key[4, 0] *= 0.001
-    ks, vs = torch.rand(kvh) * 0.004 + 0.004, torch.rand(kvh) * 0.004 + 0.004
+    g = torch.Generator().manual_seed(kvh)
+    ks, vs = (torch.rand(kvh, generator=g) * 0.004 + 0.004 for _ in range(2))
     empty = [torch.zeros(n + p, kvh, 128, dtype=torch.bfloat16) for n, p in zip(rows, prefix)]
     r = U.Ranges(empty, empty, "int4", ks, vs, extra=3)
     before = {n: getattr(r, n).cpu().clone() for n in ("k", "v")}
@@ -300,7 +301,8 @@ def test_rope_append(neox, rot, h, kvh, write_key):
     pos = torch.from_numpy(rs.randint(0, 300, size=n)).cuda()
     freq = torch.outer(torch.arange(300.0), 1.0 / 10000.0 ** (torch.arange(0, rot, 2) / rot))
     cs = torch.cat([freq.cos(), freq.sin()], -1).bfloat16().cuda()
-    ks, vs = torch.rand(kvh) * 0.004 + 0.006, torch.rand(kvh) * 0.004 + 0.006
+    g = torch.Generator().manual_seed(rot + kvh)
+    ks, vs = (torch.rand(kvh, generator=g) * 0.004 + 0.006 for _ in range(2))
     empty = [torch.zeros(x, kvh, 128, dtype=torch.bfloat16) for x in lens]
     i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
     starts, zero = i32([0, 5, 6, 6]), torch.zeros(4, dtype=torch.int64, device="cuda")

@@ -28,6 +28,23 @@ struct SmemOptIn {
   }
 };
 
+// Launches a kernel as a programmatic dependent of the one in front of it on the stream: its CTAs may be placed, and run
+// up to their griddepcontrol.wait, once that kernel's have all started and released it.
+template <typename K, typename P>
+inline bool launch_dependent(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, const P &p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess;
+}
+
 struct AppendParams {
   const void *key, *value;
   int64_t key_stride, value_stride;  // elements
@@ -80,6 +97,7 @@ struct AttnParams {
   // flat (persistent) schedule only
   int n_ctas;                         // grid size
   unsigned *fl_count;                 // [batch * kv-head slabs] piece tickets, zero between launches
+  unsigned *fl_group;                 // 4-bit engine: [n_ctas, 2 slots, 8] tickets of a group of pieces, likewise zero
   float *fl_part;                     // [n_ctas, 2 slots, 4 warps, 8 or 16 heads, 132] piece states
   // fused step (flat schedule only): this step's K/V rows, appended by the attention kernel itself
   const void *new_key, *new_value;    // bf16 [batch, kvh, 128]; nullptr = plain attention

@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) prompt_scores_kernel(PromptScor
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
+  if constexpr (PASS == 1) pdl_launch_dependents();   // pass 2 sets up while the last runs finish
   const uint32_t tmem = tmem_slot, my_lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
 
   const auto fetch = [&](int j) {   // tile j of the run into its stage: 128 rows of 256 bytes
@@ -114,6 +115,7 @@ __global__ void __launch_bounds__(kPsThreads, 2) prompt_scores_kernel(PromptScor
         *reinterpret_cast<uint4 *>(sm + half * kPsSlab + sw128_offset(r, c)) = v;
       }
       if constexpr (PASS == 2) {
+        pdl_wait_prior_grid();   // the statistics of pass 1
         float m = -INFINITY, l = 0.f;
         if (there) {   // two threads of a row share its runs
           const int runs = (n + p.run_keys - 1) / p.run_keys;
@@ -279,8 +281,8 @@ int launch_prompt_scores(const PromptScoreParams &p, cudaStream_t stream) {
   if (!opt1.ensure(prompt_scores_kernel<1>, kPsSmem) || !opt2.ensure(prompt_scores_kernel<2>, kPsSmem)) return VT_ERR_CUDA;
   const int blocks = (p.rows + kPsRows - 1) / kPsRows;
   prompt_scores_kernel<1><<<dim3(p.batch * p.kvh, p.runs, blocks), kPsThreads, kPsSmem, stream>>>(p);
-  prompt_scores_kernel<2><<<dim3(p.batch * p.kvh, p.runs), kPsThreads, kPsSmem, stream>>>(p);
-  return cudaGetLastError() == cudaSuccess ? VT_OK : VT_ERR_CUDA;
+  if (cudaGetLastError() != cudaSuccess) return VT_ERR_CUDA;
+  return launch_dependent(prompt_scores_kernel<2>, dim3(p.batch * p.kvh, p.runs), kPsThreads, kPsSmem, stream, p) ? VT_OK : VT_ERR_CUDA;
 }
 
 }  // namespace vt

@@ -20,6 +20,7 @@ constexpr int kAccTokens = 4;   // tokens per thread
 // grid: (entry x kv head, blocks of 1024 tokens)
 template <int G>
 __global__ void __launch_bounds__(kAccThreads) accumulate_kernel(ScoreParams p) {
+  pdl_wait_prior_grid();   // the attention kernel in front: everything below is its output or follows it
   const int b = blockIdx.x / p.kvh, head = blockIdx.x % p.kvh;
   const int len = min(p.seq_lens[b], p.logit_rows);
   const int t0 = blockIdx.y * kAccThreads * kAccTokens + threadIdx.x;
@@ -59,15 +60,16 @@ __global__ void __launch_bounds__(kAccThreads) accumulate_kernel(ScoreParams p) 
 
 int launch_accumulate(const ScoreParams &p, int g, int max_seq_len, cudaStream_t stream) {
   const dim3 grid(p.batch * p.kvh, (max_seq_len + kAccThreads * kAccTokens - 1) / (kAccThreads * kAccTokens));
+  bool ok;
   switch (g) {
-    case 1: accumulate_kernel<1><<<grid, kAccThreads, 0, stream>>>(p); break;
-    case 2: accumulate_kernel<2><<<grid, kAccThreads, 0, stream>>>(p); break;
-    case 4: accumulate_kernel<4><<<grid, kAccThreads, 0, stream>>>(p); break;
-    case 8: accumulate_kernel<8><<<grid, kAccThreads, 0, stream>>>(p); break;
-    case 16: accumulate_kernel<16><<<grid, kAccThreads, 0, stream>>>(p); break;
+    case 1: ok = launch_dependent(accumulate_kernel<1>, grid, kAccThreads, 0, stream, p); break;
+    case 2: ok = launch_dependent(accumulate_kernel<2>, grid, kAccThreads, 0, stream, p); break;
+    case 4: ok = launch_dependent(accumulate_kernel<4>, grid, kAccThreads, 0, stream, p); break;
+    case 8: ok = launch_dependent(accumulate_kernel<8>, grid, kAccThreads, 0, stream, p); break;
+    case 16: ok = launch_dependent(accumulate_kernel<16>, grid, kAccThreads, 0, stream, p); break;
     default: return VT_ERR_UNSUPPORTED;
   }
-  return cudaGetLastError() == cudaSuccess ? VT_OK : VT_ERR_CUDA;
+  return ok ? VT_OK : VT_ERR_CUDA;
 }
 
 }  // namespace vt

@@ -410,23 +410,33 @@ struct Layout4 {
   static_assert(kPiece % 8 == 0 && kQ % 16 == 0 && kAt % 16 == 0 && kMeta % 8 == 0, "alignment");
 };
 
-// Merge of one kv head of a stream by the warp that drew its last ticket (scratch layout of merge_stream, but a ticket
-// counter per head and no meeting of the CTA's warps: the heads of a stream are then merged by whichever CTAs finish
-// last, side by side; one CTA doing all of them took 12 of a 21 us call over 700 rows of 32/8 heads, its reads of
-// 370 KB alone).  Four q heads at a time with sixteen 16-byte rows in flight, the first before the weights are known.
-template <int U, int R, int HEADS>
-__device__ __noinline__ void merge_head(const AttnParams &p, int b, int kv_head, int stream_begin, long long total, int n_ctas,
-                                        int c_first, int c_last, int lane, int g) {
-  constexpr int I = 4, J = 4;
-  const int n_src = (c_last - c_first + 1) * R, hh = kv_head % U;
-  const int slot0 = stream_begin <= total * c_first / n_ctas ? 0 : 1;   // later CTAs start inside the stream: slot 0
-  const auto row = [&](int i, int head) -> const float * {
-    const int c = i / R, r = i % R;
-    const size_t slot = static_cast<size_t>(c_first + c) * 2 + (c == 0 ? slot0 : 0);
-    return p.fl_part + ((slot * kCWarps + r * U + hh) * HEADS + head) * kPartRow;
+// Merging the pieces of a stream.  Every warp publishes its own state (the scratch layout of merge_stream) and draws a
+// ticket of its kv head; whoever draws the last one merges, so the heads of a stream are merged side by side by whichever
+// CTAs finish last.  A stream cut into many states is merged in two levels: groups of about sqrt(states), each by the
+// warp that completes it, into the state of the group's first piece; then the groups.  One level cost 60 us with the 296
+// states that one long sequence of 8 kv heads leaves, and 100 us where four warps share a head.
+struct MergeArgs {
+  int b, kv_head, first, count, step, per;   // pieces first, first + step, ... (count of them), `per` states each
+  int c_first, slot0;                        // the stream's first piece and its scratch slot
+};
+
+// I q heads at a time, J states of each in flight, the first before the weights are known.  final: the result; otherwise
+// the merged state goes to the first piece's first row.  One warp alone issues an instruction every few cycles, so what
+// counts is their number: a lane works out where one state lies and the others take it from there by a shuffle (with the
+// division in every load 22 states of 4 heads took 21 us).  Rows of heads behind the last and the repeated last state
+// are read along, and left out or weighted 0.
+template <int U, int HEADS, int I, int J>
+__device__ __forceinline__ void merge_states(const AttnParams &p, const MergeArgs &a, bool final, int lane, int g) {
+  const int n_src = a.count * a.per, hh = a.kv_head % U;
+  const auto state_at = [&](int i) {   // in floats; the scratch holds below 2^25
+    const int q = i / a.per, c = a.first + q * a.step, r = i - q * a.per;
+    const int slot = c * 2 + (c == a.c_first ? a.slot0 : 0);
+    return (slot * kCWarps + r * U + hh) * (HEADS * kPartRow);
   };
-  const float vsc = __ldg(p.v_scale + kv_head);
+  const float vsc = __ldg(p.v_scale + a.kv_head);
+  float *const part = p.fl_part;
   for (int h0 = 0; h0 < g; h0 += I) {
+    const float *const mine = part + h0 * kPartRow + lane * 4;
     float M[I], L[I];
     float4 acc[I];
 #pragma unroll
@@ -435,27 +445,26 @@ __device__ __noinline__ void merge_head(const AttnParams &p, int b, int kv_head,
       L[k] = 0.f;
       acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const int n_heads = min(I, g - h0);
     for (int s0 = 0; s0 < n_src; s0 += 32) {
       const int cnt = min(32, n_src - s0);
+      const int at = state_at(s0 + min(lane, cnt - 1));
       float2 ml[I];
 #pragma unroll
       for (int k = 0; k < I; ++k) {
-        ml[k] = make_float2(-INFINITY, 0.f);
-        if (lane < cnt && k < n_heads) ml[k] = __ldcg(reinterpret_cast<const float2 *>(row(s0 + lane, h0 + k) + 128));
+        ml[k] = __ldcg(reinterpret_cast<const float2 *>(part + at + (h0 + k) * kPartRow + 128));
+        if (lane >= cnt) ml[k] = make_float2(-INFINITY, 0.f);
       }
       float4 v[J][I];
       const auto fetch = [&](int j0) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+        for (int j = 0; j < J; ++j) {
+          const float *src = mine + __shfl_sync(0xffffffffu, at, j0 + j);
 #pragma unroll
-          for (int k = 0; k < I; ++k) {
-            v[j][k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (k < n_heads && j0 + j < cnt) v[j][k] = __ldcg(reinterpret_cast<const float4 *>(row(s0 + j0 + j, h0 + k)) + lane);
-          }
+          for (int k = 0; k < I; ++k) v[j][k] = __ldcg(reinterpret_cast<const float4 *>(src + k * kPartRow));
+        }
       };
       fetch(0);
-      float w[I];   // weight of source s0 + lane
+      float w[I];   // weight of state s0 + lane
 #pragma unroll
       for (int k = 0; k < I; ++k) {
         float mx = ml[k].x;
@@ -470,31 +479,87 @@ __device__ __noinline__ void merge_head(const AttnParams &p, int b, int kv_head,
         acc[k].x *= f; acc[k].y *= f; acc[k].z *= f; acc[k].w *= f;
         M[k] = Mn;
       }
+#pragma unroll 1
       for (int j0 = 0; j0 < cnt; j0 += J) {
         if (j0 > 0) fetch(j0);
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
           for (int k = 0; k < I; ++k) {
-            const float y = __shfl_sync(0xffffffffu, w[k], (j0 + j) & 31);   // 0 behind the last source
+            const float y = __shfl_sync(0xffffffffu, w[k], j0 + j);   // 0 behind the last state
             acc[k].x = fmaf(y, v[j][k].x, acc[k].x); acc[k].y = fmaf(y, v[j][k].y, acc[k].y);
             acc[k].z = fmaf(y, v[j][k].z, acc[k].z); acc[k].w = fmaf(y, v[j][k].w, acc[k].w);
           }
       }
     }
+    __syncwarp();   // every lane has read the rows of these heads
 #pragma unroll
     for (int k = 0; k < I; ++k) {
-      if (k < n_heads) {
-        const int hq = kv_head * g + h0 + k;
+      if (h0 + k >= g) continue;
+      if (final) {
+        const int hq = a.kv_head * g + h0 + k;
         const float inv = vsc / L[k];
         uint2 packed;
         packed.x = pack_bf16(acc[k].x * inv, acc[k].y * inv);
         packed.y = pack_bf16(acc[k].z * inv, acc[k].w * inv);
-        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + b * p.out_stride + hq * kHeadDim + lane * 4) = packed;
-        if (lane == 0) write_stats(p, b * p.h + hq, M[k], L[k]);
+        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p.out) + a.b * p.out_stride + hq * kHeadDim + lane * 4) = packed;
+        if (lane == 0) write_stats(p, a.b * p.h + hq, M[k], L[k]);
+      } else {
+        float *dst = part + state_at(0) + (h0 + k) * kPartRow;
+        *reinterpret_cast<float4 *>(dst + lane * 4) = acc[k];
+        if (lane == 0) *reinterpret_cast<float2 *>(dst + 128) = make_float2(M[k], L[k]);
       }
     }
   }
+}
+template <int U, int HEADS>
+__device__ __noinline__ void merge_any(const AttnParams &p, const MergeArgs &a, bool final, int lane, int g) {
+  if (g == 1) merge_states<U, HEADS, 1, 16>(p, a, final, lane, g);
+  else if (g == 2) merge_states<U, HEADS, 2, 8>(p, a, final, lane, g);
+  else merge_states<U, HEADS, 4, 4>(p, a, final, lane, g);
+}
+
+// owner_of with a division of 32 bits where that is enough (64 bits: some 300 cycles each, between a state and its merge).
+__device__ __forceinline__ int owner4(int tau, int total, int n_ctas) {
+  const unsigned long long x = static_cast<unsigned long long>(tau + 1) * n_ctas - 1;
+  return static_cast<int>(x >> 32 ? x / total : static_cast<unsigned>(x) / static_cast<unsigned>(total));
+}
+
+// One ticket for the whole warp, whose stores come before it; true for the last of `n`, which also clears the counter.
+__device__ __forceinline__ bool last_ticket(unsigned *ctr, int n, int lane) {
+  __syncwarp();
+  int last = 0;
+  if (lane == 0) {   // the fence covers the stores of the lanes it has met
+    __threadfence();
+    last = atomicAdd(ctr, 1u) + 1 == static_cast<unsigned>(n);
+    if (last) *ctr = 0u;   // clean for the next launch
+    __threadfence();
+  }
+  return __shfl_sync(0xffffffffu, last, 0);
+}
+
+// Called by every warp after it has published its state of piece `c` of stream [c_first, c_last].
+constexpr int kOneLevel = 48;   // states; a second level costs its tickets and its start, about 4 us
+template <int U, int R, int HEADS>
+__device__ __noinline__ void publish(const AttnParams &p, int b, int kv_head, int c, int c_first, int c_last, int slot0, int lane, int g) {
+  const int pieces = c_last - c_first + 1, hh = kv_head % U;
+  unsigned *ctr = p.fl_count + b * p.kvh + kv_head;
+  MergeArgs a{b, kv_head, c_first, pieces, 1, R, c_first, slot0};
+  int n = pieces * R;
+  if (n > kOneLevel) {
+    const int size = (static_cast<int>(sqrtf(static_cast<float>(n))) + R - 1) / R;   // pieces per group
+    const int k = (c - c_first) / size, lead = c_first + k * size;
+    const size_t slot = static_cast<size_t>(lead) * 2 + (lead == c_first ? slot0 : 0);
+    a.first = lead;
+    a.count = min(size, c_last + 1 - lead);
+    if (!last_ticket(p.fl_group + slot * kCWarps + hh, a.count * R, lane)) return;
+    merge_any<U, HEADS>(p, a, false, lane, g);
+    a.first = c_first;
+    a.count = n = (pieces + size - 1) / size;
+    a.step = size;
+    a.per = 1;
+  }
+  if (last_ticket(ctr, n, lane)) merge_any<U, HEADS>(p, a, true, lane, g);
 }
 
 // Looks up the next pieces of positions [meta[3], end), one warp for the CTA: meta[2] = how many that hold tiles, meta[3]
@@ -605,8 +670,8 @@ __device__ __forceinline__ void next_copy(const PieceRec *rec, int pieces, int &
 }
 
 // Piece `now` of the CTA's share, the `it`-th tile on: attention, then either the result or a published state and a
-// ticket.  Bit 0: a bounded wait ran out; bit 1: this warp drew the last ticket of its head.  A function of its own, with
-// no calls inside: what the compiler would otherwise keep on the stack across the merge it reloads in the tile loop.
+// ticket.  Bit 0: a bounded wait ran out; bit 1: a state was published.  A function of its own, with no calls inside: what
+// the compiler would otherwise keep on the stack across the merge it reloads in the tile loop.
 template <int U, int NB, bool LOG>
 __device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, int state, int &copy_piece, int &copy_tile) {
   using C = Cfg4<U>;
@@ -697,20 +762,7 @@ __device__ __noinline__ int run_piece(const AttnParams &p, int now, int it, int 
     if (p.overlap) pdl_wait_prior_grid();   // the scratch is shared with the previous launch
     float *slot_base = p.fl_part + (static_cast<size_t>(blockIdx.x) * 2 + (state & 4 ? 0 : 1)) * kCWarps * HEADS * kPartRow;
     st.template store<kPartRow>(slot_base + warp * HEADS * kPartRow, lane, g);
-    const long long total = meta[0];
-    const int n_ctas = meta[1];
-    const int c_first = owner_of(pc.stream_begin + kBoundaryCost, total, n_ctas);
-    const int c_last = owner_of(pc.stream_end - 1, total, n_ctas);
-    __syncwarp();
-    int last = 0;
-    if (lane == 0) {   // one ticket per warp; the fence covers the stores of the lanes it has met
-      __threadfence();
-      unsigned *ctr = p.fl_count + pc.b * p.kvh + kv_head;
-      last = atomicAdd(ctr, 1u) + 1 == static_cast<unsigned>((c_last - c_first + 1) * R);
-      if (last) *ctr = 0u;   // clean for the next launch
-      __threadfence();
-    }
-    return (failed ? 1 : 0) | (__shfl_sync(0xffffffffu, last, 0) << 1);
+    return (failed ? 1 : 0) | 2;
   }
   return failed ? 1 : 0;
 }
@@ -806,10 +858,10 @@ __global__ void __launch_bounds__(kThreads4, NB == 1 ? 2 : 1) attn_int4_kernel(c
       first = false;
       it += pc.tile_end - pc.tile_begin;
       if (got & 2) {
-        const long long total = meta[0];
-        const int n_ctas = meta[1];
-        merge_head<U, R, HEADS>(p, pc.b, pc.slab * U + hs, pc.stream_begin, total, n_ctas,
-                                owner_of(pc.stream_begin + kBoundaryCost, total, n_ctas), owner_of(pc.stream_end - 1, total, n_ctas), lane, g);
+        const int total = meta[0], n_ctas = meta[1], c_first = owner4(pc.stream_begin + kBoundaryCost, total, n_ctas);
+        // the stream is its first CTA's first piece iff it already runs where that CTA's share begins
+        const int slot0 = static_cast<long long>(pc.stream_begin) * n_ctas <= static_cast<long long>(total) * c_first ? 0 : 1;
+        publish<U, R, HEADS>(p, pc.b, pc.slab * U + hs, blockIdx.x, c_first, owner4(pc.stream_end - 1, total, n_ctas), slot0, lane, g);
       }
       // a stream that lies wholly in this CTA's share used slot 1, as the next piece may
       if (R > 1 && pc.tile_begin == 0 && pc.tile_end == pc.tiles) named_bar_sync(1, kCWarps * 32);

@@ -67,8 +67,9 @@ size_t attn_workspace_bytes(int batch, int h, int max_parts) {
   return kStatusBytes + ml + rows * kHeadDim * sizeof(float);
 }
 
+// Ticket counters of the streams, then those of the 4-bit engine's groups of pieces.
 static size_t flat_counter_bytes(int batch, int kvh) {
-  return (static_cast<size_t>(batch) * kvh * sizeof(unsigned) + 255) / 256 * 256;
+  return (static_cast<size_t>(batch) * kvh * sizeof(unsigned) + 255) / 256 * 256 + kFlatMaxCtas * 2 * 8 * sizeof(unsigned);
 }
 static size_t flat_workspace_bytes(int batch, int h, int kvh, int kv_dtype, bool worst_case = false) {
   const int heads = (!worst_case && (h / kvh) <= 8) ? 8 : 16;
@@ -97,6 +98,7 @@ static void carve_flat(void *ws, int batch, int kvh, AttnParams *p) {
   char *c = static_cast<char *>(ws);
   p->status = reinterpret_cast<uint32_t *>(c);
   p->fl_count = reinterpret_cast<unsigned *>(c + kStatusBytes);
+  p->fl_group = p->fl_count + (static_cast<size_t>(batch) * kvh + 63) / 64 * 64;
   p->fl_part = reinterpret_cast<float *>(c + kStatusBytes + flat_counter_bytes(batch, kvh));
 }
 
@@ -301,7 +303,8 @@ static int decode_attn_impl(void *out, int64_t out_stride, const void *q, int64_
     // the caller guarantees a zero-initialised buffer instead, or when the caller
     // gives that guarantee for an ordinary launch (VT_STEP_CLEAN_SCRATCH).
     if (!p.overlap && !(flags & VT_STEP_CLEAN_SCRATCH) &&
-        cudaMemsetAsync(p.fl_count, 0, static_cast<size_t>(batch) * kvh * sizeof(unsigned), s) != cudaSuccess)
+        cudaMemsetAsync(p.fl_count, 0, kv_dtype == VT_KV_INT4 ? vt::flat_counter_bytes(batch, kvh)
+                                                              : static_cast<size_t>(batch) * kvh * sizeof(unsigned), s) != cudaSuccess)
       return VT_ERR_CUDA;
     // fp8 ranges with tensor maps: the tcgen05 engine where the shape allows (same schedule, same scratch)
     if (maps && kv_dtype == VT_KV_FP8_E4M3 && vt::attn_flat_umma_supports(batch, h, kvh, kv_dtype)) {

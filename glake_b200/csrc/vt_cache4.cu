@@ -4,8 +4,9 @@
 // Bytes per (row, kv head): append reads 512 (K and V, bf16) and writes 136; read-back the reverse.  HBM is the bound
 // only if the arithmetic stays small, about 14 instructions per element at the copy bandwidth.  Hence eight lanes per
 // (row, head) with 16 elements each, the group maximum on packed bf16, and one multiplication by 1 / step per element
-// in place of a division (append_int4_kernel); 8 x 4096 rows of 8 heads: append 140 -> 63 us, read-back 44 ->
-// 36 us against one warp per (row, head) with a division per element.
+// in place of a division (append_int4_kernel), with the loads a round ahead; 8 x 4096 rows of 8 heads: append 44 us (3.9
+// TB/s), read-back 33 us (5.1 TB/s), against 140 and 44 with one warp per (row, head) and a division per element.  What
+// bounds the append is instruction issue (82 % busy), the integer unit (60 %) the read-back.
 #include <algorithm>
 
 #include "../../include/vtensor.h"

@@ -5,6 +5,8 @@
 // (entry, q head); this kernel turns them into weights.  The weight of a row needs the sum over ALL rows, which no CTA
 // of the attention launch knows while it holds the logits, so a second pass is needed either way; re-reading K for it
 // would cost 256 bytes per (row, kv head), the logits cost 8 g.  Bytes: 4 g + 8 per (row, kv head).
+// Measured, whole call: bf16, 8 sequences of 512-2048 rows, 32/32 heads 41 us; 32 of 4k-16k, 8/1 heads 49; fp8, 64 of
+// 2k-8k, 32/8 heads 158, of which the accumulation 6, 9 and 13 (it starts while the attention kernel drains).
 #include <algorithm>
 
 #include "../../include/vtensor.h"

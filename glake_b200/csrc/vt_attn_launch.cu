@@ -67,15 +67,20 @@ size_t attn_workspace_bytes(int batch, int h, int max_parts) {
   return kStatusBytes + ml + rows * kHeadDim * sizeof(float);
 }
 
-// Ticket counters of the streams, then those of the 4-bit engine's groups of pieces.
-static size_t flat_counter_bytes(int batch, int kvh) {
-  return (static_cast<size_t>(batch) * kvh * sizeof(unsigned) + 255) / 256 * 256 + kFlatMaxCtas * 2 * 8 * sizeof(unsigned);
+// Tickets of the 4-bit engine's groups of pieces, in front of those of the streams.
+constexpr size_t kGroupBytes = kFlatMaxCtas * 2 * 8 * sizeof(unsigned);
+static_assert(kGroupBytes % 256 == 0, "alignment");
+// The 4-bit engine keeps room for the largest batch: a call that runs in parts, or calls of several batch sizes, then
+// never leave states where the next one expects clean counters.
+static size_t flat_counter_bytes(int batch, int kvh, bool int4) {
+  const size_t streams = static_cast<size_t>(int4 ? kFlatMaxBatch : batch) * kvh * sizeof(unsigned);
+  return (int4 ? kGroupBytes : 0) + (streams + 255) / 256 * 256;
 }
 static size_t flat_workspace_bytes(int batch, int h, int kvh, int kv_dtype, bool worst_case = false) {
   const int heads = (!worst_case && (h / kvh) <= 8) ? 8 : 16;
   const int warps = worst_case ? 8 : flat_consumer_warps(kv_dtype);   // 4-bit: 8, as fp8
   const int ctas = worst_case ? kFlatMaxCtas : flat_max_ctas(h, kvh, kv_dtype);
-  return kStatusBytes + flat_counter_bytes(batch, kvh) +
+  return kStatusBytes + std::max(flat_counter_bytes(batch, kvh, kv_dtype == VT_KV_INT4), worst_case ? flat_counter_bytes(batch, kvh, true) : 0) +
          static_cast<size_t>(ctas) * 2 * warps * heads * kFlatPartRow * sizeof(float);
 }
 
@@ -94,12 +99,12 @@ void carve_workspace(void *ws, int batch, int h, int max_parts, AttnParams *p) {
   p->ws_o = reinterpret_cast<float *>(c + kStatusBytes + (rows * 2 * sizeof(float) + 255) / 256 * 256);
 }
 
-static void carve_flat(void *ws, int batch, int kvh, AttnParams *p) {
+static void carve_flat(void *ws, int batch, int kvh, bool int4, AttnParams *p) {
   char *c = static_cast<char *>(ws);
   p->status = reinterpret_cast<uint32_t *>(c);
-  p->fl_count = reinterpret_cast<unsigned *>(c + kStatusBytes);
-  p->fl_group = p->fl_count + (static_cast<size_t>(batch) * kvh + 63) / 64 * 64;
-  p->fl_part = reinterpret_cast<float *>(c + kStatusBytes + flat_counter_bytes(batch, kvh));
+  p->fl_group = reinterpret_cast<unsigned *>(c + kStatusBytes);
+  p->fl_count = reinterpret_cast<unsigned *>(c + kStatusBytes + (int4 ? kGroupBytes : 0));
+  p->fl_part = reinterpret_cast<float *>(c + kStatusBytes + flat_counter_bytes(batch, kvh, int4));
 }
 
 int plan_attn(int batch, int h, int kvh, int max_seq_len, int kv_dtype, int num_splits, AttnPlan *plan) {
@@ -293,7 +298,7 @@ static int decode_attn_impl(void *out, int64_t out_stride, const void *q, int64_
       p.new_key = new_key; p.new_value = new_value;
       p.new_key_stride = new_key_stride; p.new_value_stride = new_value_stride; p.byte_off = byte_off;
     }
-    vt::carve_flat(workspace, batch, kvh, &p);
+    vt::carve_flat(workspace, batch, kvh, kv_dtype == VT_KV_INT4, &p);
     // Overlap only for the fused launch: a separate append kernel in front of this one
     // writes the row this launch reads, and only ordinary stream order covers that.
     p.overlap = !fused ? 0 : (flags & VT_STEP_EARLY_KV) ? 2 : (flags & VT_STEP_OVERLAP) ? 1 : 0;
@@ -303,8 +308,8 @@ static int decode_attn_impl(void *out, int64_t out_stride, const void *q, int64_
     // the caller guarantees a zero-initialised buffer instead, or when the caller
     // gives that guarantee for an ordinary launch (VT_STEP_CLEAN_SCRATCH).
     if (!p.overlap && !(flags & VT_STEP_CLEAN_SCRATCH) &&
-        cudaMemsetAsync(p.fl_count, 0, kv_dtype == VT_KV_INT4 ? vt::flat_counter_bytes(batch, kvh)
-                                                              : static_cast<size_t>(batch) * kvh * sizeof(unsigned), s) != cudaSuccess)
+        cudaMemsetAsync(p.fl_group, 0, (kv_dtype == VT_KV_INT4 ? vt::kGroupBytes : 0) + static_cast<size_t>(batch) * kvh * sizeof(unsigned),
+                        s) != cudaSuccess)
       return VT_ERR_CUDA;
     // fp8 ranges with tensor maps: the tcgen05 engine where the shape allows (same schedule, same scratch)
     if (maps && kv_dtype == VT_KV_FP8_E4M3 && vt::attn_flat_umma_supports(batch, h, kvh, kv_dtype)) {

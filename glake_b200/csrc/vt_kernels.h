@@ -97,7 +97,7 @@ struct AttnParams {
   // flat (persistent) schedule only
   int n_ctas;                         // grid size
   unsigned *fl_count;                 // [batch * kv-head slabs] piece tickets, zero between launches
-  unsigned *fl_group;                 // 4-bit engine: [n_ctas, 2 slots, 8] tickets of a group of pieces, likewise zero
+  unsigned *fl_group;                 // 4-bit engine: [CTAs, 2 slots, 8] tickets of a group of pieces, likewise zero
   float *fl_part;                     // [n_ctas, 2 slots, 4 warps, 8 or 16 heads, 132] piece states
   // fused step (flat schedule only): this step's K/V rows, appended by the attention kernel itself
   const void *new_key, *new_value;    // bf16 [batch, kvh, 128]; nullptr = plain attention

@@ -258,6 +258,29 @@ def test_fused_steps(h, kvh):
             assert bool(((o[i].double() - want).abs() <= tol).all())
 
 
+def test_steps_over_one_clean_workspace():
+    """One zero-filled workspace for steps of different batch sizes, one of them beyond the schedule's table: every call
+    finds its counters clean (same result, bit for bit, as with a buffer that is cleared for the call)."""
+    from glake_b200 import ops
+    h, kvh = 8, 2
+    lens = [2600, 1300] + [1 + 7 * i % 90 for i in range(1028)]
+    k, v, ks, vs, rs = make(5, lens, kvh)
+    r = U.Ranges([x[:-1] for x in k], [x[:-1] for x in v], "int4", ks, vs)
+    ws = ops.new_workspace(torch.device("cuda"), len(lens), h, 128, max(lens))
+    key, value, q = (normal_bf16(rs, len(lens), n, 128).cuda() for n in (kvh, kvh, h))
+    off = torch.tensor([(n - 1) * r.row for n in lens]).cuda()
+    seq_lens = torch.tensor(lens, dtype=torch.int32).cuda()
+
+    def step(n, **how):
+        out = torch.zeros(n, h, 128, dtype=torch.bfloat16, device="cuda")
+        ops.decode_step(out, q[:n], key[:n], value[:n], r.k_table.data_ptr(), r.v_table.data_ptr(), off[:n], r.slot_ids[:n],
+                        seq_lens[:n], max(lens), kvh, 128 ** -0.5, "int4", ks.cuda(), vs.cuda(), **how)
+        return out.cpu()
+
+    for n in (1, len(lens), 2, len(lens), len(lens), 40):
+        assert torch.equal(step(n, workspace=ws, clean_scratch=True), step(n))
+
+
 def test_captured_and_replayed_on_another_stream():
     from glake_b200 import ops
     lens, h, kvh = [700, 33], 32, 8

@@ -99,6 +99,14 @@ void carve_workspace(void *ws, int batch, int h, int max_parts, AttnParams *p) {
   p->ws_o = reinterpret_cast<float *>(c + kStatusBytes + (rows * 2 * sizeof(float) + 255) / 256 * 256);
 }
 
+// Clears `n` 16-byte words in front of the 4-bit kernel, which is launched behind it as a dependent: it starts at once and
+// waits only before it publishes a state (one sequence of 700 rows: 24.7 us with a memset in its place, 21.8 so).
+__global__ void __launch_bounds__(256) clear_tickets_kernel(uint4 *p, int n) {
+  pdl_launch_dependents();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 static void carve_flat(void *ws, int batch, int kvh, bool int4, AttnParams *p) {
   char *c = static_cast<char *>(ws);
   p->status = reinterpret_cast<uint32_t *>(c);
@@ -307,10 +315,15 @@ static int decode_attn_impl(void *out, int64_t out_stride, const void *q, int64_
     // in overlap mode, where a memset between the kernels would serialise them and
     // the caller guarantees a zero-initialised buffer instead, or when the caller
     // gives that guarantee for an ordinary launch (VT_STEP_CLEAN_SCRATCH).
-    if (!p.overlap && !(flags & VT_STEP_CLEAN_SCRATCH) &&
-        cudaMemsetAsync(p.fl_group, 0, (kv_dtype == VT_KV_INT4 ? vt::kGroupBytes : 0) + static_cast<size_t>(batch) * kvh * sizeof(unsigned),
-                        s) != cudaSuccess)
+    const bool clear = !p.overlap && !(flags & VT_STEP_CLEAN_SCRATCH);
+    if (clear && kv_dtype == VT_KV_INT4) {
+      const int words = static_cast<int>((vt::kGroupBytes + static_cast<size_t>(batch) * kvh * sizeof(unsigned) + 15) / 16);
+      vt::clear_tickets_kernel<<<(words + 255) / 256, 256, 0, s>>>(reinterpret_cast<uint4 *>(p.fl_group), words);
+      if (cudaGetLastError() != cudaSuccess) return VT_ERR_CUDA;
+      p.overlap = 1;   // over that kernel, which itself follows everything before it
+    } else if (clear && cudaMemsetAsync(p.fl_count, 0, static_cast<size_t>(batch) * kvh * sizeof(unsigned), s) != cudaSuccess) {
       return VT_ERR_CUDA;
+    }
     // fp8 ranges with tensor maps: the tcgen05 engine where the shape allows (same schedule, same scratch)
     if (maps && kv_dtype == VT_KV_FP8_E4M3 && vt::attn_flat_umma_supports(batch, h, kvh, kv_dtype)) {
       p.maps = maps;
